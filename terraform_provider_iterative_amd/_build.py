@@ -204,8 +204,11 @@ def build_hip(force: bool = False, verbose: bool = False) -> str:
     srcs = _sources("hip/*.hip", "hip/*.cpp")
     headers = _sources("hip/*.h", "common/*.h")
     tl = torch_lib_dir()
+    # no packed fp32 instructions (v_pk_add/mul/fma_f32): hipcc makes them from ordinary float
+    # code, and some of their forms have given wrong results on these GPUs without any error
     flags = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall",
-             "-Wno-unused-function", "-munsafe-fp-atomics", _define_version()]
+             "-Wno-unused-function", "-munsafe-fp-atomics",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", _define_version()]
     objdir = os.path.join(LIB, "obj")
     os.makedirs(objdir, exist_ok=True)
 
