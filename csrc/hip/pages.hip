@@ -1,0 +1,515 @@
+// Pages of a paged cache: copying, forking, freeing and compacting (ops/paging.py).
+//
+// A pool is a set of tensors whose first dimension is the page (keys and values of every layer)
+// and int32 bookkeeping on the device: table[slot][k] = page of tokens [k P, (k + 1) P) of the
+// slot's sequence, refs[page] = table entries that name it, and a bit per page that has none.
+// Nothing here waits for the host: numbers of pages to move are read on the device, so a step
+// that forks and frees can be captured into a graph.
+//
+// Order: free pages are taken lowest number first, slots in the order they are asked for, and
+// reference counts and bits are changed by integer atomics only, so that every result is the same
+// on every run -- and on the host implementation (csrc/native/pages.cpp).
+//
+//  k_reserve      one workgroup: checks a fork or an extension as a whole, then takes its pages
+//                 from the free bits (1024 words at a time: popcount, prefix sum)
+//  k_fork         table rows of the forks, and their partial pages' bytes
+//  k_free         a workgroup per slot
+//  k_plan         one workgroup: holes and movers of a compaction, and the pages to clear
+//  k_compact      table entries, moved pages' bytes
+//  k_clear        free pages' bytes
+//  k_copy         pages named by the caller
+#include <hip/hip_runtime.h>
+
+#include "internal.h"
+#include "tpi_hip.h"
+
+namespace {
+
+constexpr int kBlock = 256;   // threads that move bytes
+constexpr int kPlan = 1024;   // threads of the one-workgroup kernels
+constexpr int kRowSpan = 1024;  // table entries of a row that one workgroup of k_fork takes
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// scratch: [pages] x 4, [slots] x 5
+__device__ static inline int32_t* list(const tpi_pages& p, int i) {
+  return p.scratch + (int64_t)i * p.pages;
+}
+__device__ static inline int32_t* slot_list(const tpi_pages& p, int i) {
+  return p.scratch + 4 * (int64_t)p.pages + (int64_t)i * p.slots;
+}
+enum { TAKEN = 0, HOLES = 0, MOVERS = 1, CLEARS = 2, MAP = 3 };            // list()
+enum { MARK = 0, OFFSET = 1, LENGTH = 2, PAIR_SRC = 3, PAIR_DST = 4 };     // slot_list()
+
+__device__ static inline int64_t number(const void* a, int64_t i, bool wide) {
+  return wide ? ((const int64_t*)a)[i] : ((const int32_t*)a)[i];
+}
+
+__device__ static inline void refuse(const tpi_pages& p, int code) {
+  atomicCAS(&p.header[TPI_PAGES_ERROR], 0, code);
+}
+
+__device__ static inline int32_t pages_of(int64_t tokens, int32_t per) {
+  return (int32_t)((tokens + per - 1) / per);
+}
+
+// ---- moving bytes ------------------------------------------------------------------------------
+
+// The tensor of chunk c of a page (chunk0 ascends).
+__device__ static inline const tpi_page_tensor& tensor_of(const tpi_pages& p, uint32_t c) {
+  int lo = 0, hi = p.ntensors - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.tensors[mid].chunk0 <= c) lo = mid; else hi = mid - 1;
+  }
+  return p.tensors[lo];
+}
+
+template <typename T, typename F>
+__device__ static inline void over_chunk(const tpi_page_tensor& t, uint32_t chunk, F f) {
+  const uint64_t total = (uint64_t)t.rows * t.row_units;
+#pragma unroll
+  for (int k = 0; k < TPI_PAGE_UNITS / kBlock; ++k) {
+    const uint64_t u = (uint64_t)chunk * TPI_PAGE_UNITS + k * kBlock + threadIdx.x;
+    if (u >= total) continue;
+    uint64_t row = 0, col = u;
+    if (t.rows > 1) {
+      row = u / t.row_units;
+      col = u - row * t.row_units;
+    }
+    f((int64_t)row * t.row_stride + (int64_t)col * (int64_t)sizeof(T));
+  }
+}
+
+template <typename T>
+__device__ static inline void copy_units(const tpi_page_tensor& t, uint32_t chunk, int64_t src,
+                                         int64_t dst) {
+  const uint8_t* s = (const uint8_t*)t.base + src * t.page_stride;
+  uint8_t* d = (uint8_t*)t.base + dst * t.page_stride;
+  over_chunk<T>(t, chunk, [&](int64_t at) { *(T*)(d + at) = *(const T*)(s + at); });
+}
+
+template <typename T>
+__device__ static inline void zero_units(const tpi_page_tensor& t, uint32_t chunk, int64_t page) {
+  uint8_t* d = (uint8_t*)t.base + page * t.page_stride;
+  over_chunk<T>(t, chunk, [&](int64_t at) { *(T*)(d + at) = T{}; });
+}
+
+// Chunk c (over all tensors) of a page.
+__device__ static void copy_chunk(const tpi_pages& p, uint32_t c, int64_t src, int64_t dst) {
+  const tpi_page_tensor& t = tensor_of(p, c);
+  const uint32_t chunk = c - t.chunk0;
+  switch (t.unit) {
+    case 16: copy_units<u32x4>(t, chunk, src, dst); break;
+    case 8: copy_units<u32x2>(t, chunk, src, dst); break;
+    case 4: copy_units<uint32_t>(t, chunk, src, dst); break;
+    case 2: copy_units<uint16_t>(t, chunk, src, dst); break;
+    default: copy_units<uint8_t>(t, chunk, src, dst); break;
+  }
+}
+
+__device__ static void zero_chunk(const tpi_pages& p, uint32_t c, int64_t page) {
+  const tpi_page_tensor& t = tensor_of(p, c);
+  const uint32_t chunk = c - t.chunk0;
+  switch (t.unit) {
+    case 16: zero_units<u32x4>(t, chunk, page); break;
+    case 8: zero_units<u32x2>(t, chunk, page); break;
+    case 4: zero_units<uint32_t>(t, chunk, page); break;
+    case 2: zero_units<uint16_t>(t, chunk, page); break;
+    default: zero_units<uint8_t>(t, chunk, page); break;
+  }
+}
+
+__global__ __launch_bounds__(kBlock) void k_copy(tpi_pages p, const void* src, const void* dst,
+                                                 int64_t n, bool wide) {
+  const int64_t work = n * p.chunks;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int64_t i = w / p.chunks;
+    const int64_t s = number(src, i, wide), d = number(dst, i, wide);
+    if (s < 0 || s >= p.pages || d < 0 || d >= p.pages) {
+      if (threadIdx.x == 0) refuse(p, TPI_PAGES_EPAGE);
+      continue;
+    }
+    copy_chunk(p, (uint32_t)(w - i * p.chunks), s, d);
+  }
+}
+
+// ---- one-workgroup helpers ---------------------------------------------------------------------
+
+// Exclusive prefix sum over the kPlan threads of the workgroup; `total` = the sum.
+__device__ static inline int scan(int v, int* total) {
+  __shared__ int waves[kPlan / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < kPlan / 64; ++w) {
+    if (w < wave) before += waves[w];
+    sum += waves[w];
+  }
+  *total = sum;
+  return before + x - v;
+}
+
+// Numbers of the set bits of `bits` (page 32 w + bit) that have rank lo, lo + 1, ... below
+// `limit`, in ascending order; returns the bits that were taken.
+__device__ static inline uint32_t emit(uint32_t bits, int w, int lo, int limit, int32_t* out) {
+  uint32_t taken = 0;
+  while (bits && lo < limit) {
+    const int b = __ffs(bits) - 1;
+    out[lo++] = 32 * w + b;
+    taken |= 1u << b;
+    bits &= bits - 1;
+  }
+  return taken;
+}
+
+// Pages of slot entry i that a fork / an extension takes.
+template <bool FORK>
+__device__ static inline int32_t needed(const tpi_pages& p, const void* a, int64_t i, bool wide) {
+  const int32_t len = slot_list(p, LENGTH)[i];
+  if (FORK) return len % p.tokens != 0;
+  return pages_of(len, p.tokens) - pages_of(p.lengths[number(a, i, wide)], p.tokens);
+}
+
+template <bool FORK>
+__global__ __launch_bounds__(kPlan) void k_reserve(tpi_pages p, const void* a, const void* b,
+                                                   int n, bool wide, const void* more,
+                                                   bool more_wide, int64_t each) {
+  __shared__ int s_error;
+  __shared__ unsigned long long s_total;
+  const int tid = threadIdx.x;
+  int32_t* mark = slot_list(p, MARK);
+  int32_t* offset = slot_list(p, OFFSET);
+  int32_t* length = slot_list(p, LENGTH);
+  if (tid == 0) {
+    s_error = 0;
+    s_total = 0;
+  }
+  __syncthreads();
+  // 1. every entry by itself, and what all of them take
+  for (int i = tid; i < n; i += kPlan) {
+    const int64_t s = number(a, i, wide), d = FORK ? number(b, i, wide) : s;
+    int error = 0;
+    int64_t len = 0;
+    if (s < 0 || s >= p.slots || d < 0 || d >= p.slots) {
+      error = TPI_PAGES_ESLOT;
+    } else {
+      const int64_t old = p.lengths[s];
+      if (FORK) {
+        len = old;
+        if (s == d || p.lengths[d] != 0) error = TPI_PAGES_EBUSY;
+      } else {
+        const int64_t m = more ? number(more, i, more_wide) : each;
+        if (m < 0) {
+          error = TPI_PAGES_ETOKENS;
+        } else if (m > (int64_t)p.width * p.tokens - old || old + m > 0x7fffffff) {
+          error = TPI_PAGES_EWIDTH;
+        } else {
+          len = old + m;
+        }
+      }
+      mark[d] = i;  // of entries that name one slot, one stays
+    }
+    if (error) {
+      atomicMax(&s_error, error);
+      continue;
+    }
+    length[i] = (int32_t)len;
+    const int32_t need = FORK ? len % p.tokens != 0
+                              : pages_of(len, p.tokens) - pages_of(p.lengths[s], p.tokens);
+    if (need) atomicAdd(&s_total, (unsigned long long)need);
+  }
+  __syncthreads();
+  if (!s_error)
+    for (int i = tid; i < n; i += kPlan)
+      if (mark[FORK ? number(b, i, wide) : number(a, i, wide)] != i)
+        atomicMax(&s_error, TPI_PAGES_EDUPLICATE);
+  if (tid == 0 && s_total > (unsigned long long)p.header[TPI_PAGES_FREE])
+    atomicMax(&s_error, TPI_PAGES_ENOSPACE);
+  __syncthreads();
+  if (s_error) {
+    if (tid == 0) refuse(p, s_error);
+    if (FORK)
+      for (int i = tid; i < n; i += kPlan) length[i] = -1;  // nothing for k_fork
+    return;
+  }
+  const int total = (int)s_total;
+  // 2. where each entry's pages begin among those taken
+  for (int base = 0, carry = 0; base < n; base += kPlan) {
+    int sum;
+    const int i = base + tid;
+    const int before = scan(i < n ? needed<FORK>(p, a, i, wide) : 0, &sum);
+    if (i < n) offset[i] = carry + before;
+    carry += sum;
+  }
+  // 3. the lowest free pages
+  const int words = (p.pages + 31) / 32;
+  int found = 0;
+  for (int base = 0; base < words && found < total; base += kPlan) {
+    int sum;
+    const int w = base + tid;
+    const uint32_t bits = w < words ? p.free_bits[w] : 0;
+    const int rank = found + scan(__popc(bits), &sum);
+    if (bits && rank < total) p.free_bits[w] = bits & ~emit(bits, w, rank, total, list(p, TAKEN));
+    found += sum;
+  }
+  __syncthreads();
+  if (found < total) {  // the count and the bits disagree: not a state that these kernels leave
+    if (tid == 0) refuse(p, TPI_PAGES_ESTATE);
+    if (FORK)
+      for (int i = tid; i < n; i += kPlan) length[i] = -1;
+    return;
+  }
+  // 4. to the entries
+  const int32_t* taken = list(p, TAKEN);
+  if (FORK) {
+    for (int i = tid; i < n; i += kPlan) {
+      const int64_t s = number(a, i, wide);
+      int32_t from = -1, to = -1;
+      if (length[i] % p.tokens) {
+        from = p.table[s * p.width + length[i] / p.tokens];
+        to = taken[offset[i]];
+        p.refs[to] = 1;
+      }
+      slot_list(p, PAIR_SRC)[i] = from;
+      slot_list(p, PAIR_DST)[i] = to;
+    }
+  } else {
+    for (int r = tid; r < total; r += kPlan) {
+      int lo = 0, hi = n - 1;  // the last entry that begins at or before r
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (offset[mid] <= r) lo = mid; else hi = mid - 1;
+      }
+      const int64_t s = number(a, lo, wide);
+      p.table[s * p.width + pages_of(p.lengths[s], p.tokens) + (r - offset[lo])] = taken[r];
+      p.refs[taken[r]] = 1;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPlan) p.lengths[number(a, i, wide)] = length[i];
+  }
+  if (tid == 0) p.header[TPI_PAGES_FREE] -= total;
+}
+
+// Workgroups of one entry: `spans` for its table row, then p.chunks for its partial page.
+__global__ __launch_bounds__(kBlock) void k_fork(tpi_pages p, const void* src, const void* dst,
+                                                 int64_t n, bool wide, int spans) {
+  const int64_t per = spans + p.chunks, work = n * per;
+  for (int64_t g = blockIdx.x; g < work; g += gridDim.x) {
+    const int64_t i = g / per, j = g - i * per;
+    const int32_t len = slot_list(p, LENGTH)[i];
+    if (len < 0) return;  // refused
+    const int32_t from = slot_list(p, PAIR_SRC)[i], to = slot_list(p, PAIR_DST)[i];
+    if (j >= spans) {
+      if (from >= 0 && from < p.pages && to >= 0)
+        copy_chunk(p, (uint32_t)(j - spans), from, to);
+      continue;
+    }
+    const int64_t s = number(src, i, wide), d = number(dst, i, wide);
+    const int32_t full = len / p.tokens;
+    for (int64_t k = j * kRowSpan + threadIdx.x; k < (j + 1) * kRowSpan && k < full; k += kBlock) {
+      const int32_t page = p.table[s * p.width + k];
+      p.table[d * p.width + k] = page;
+      if (page >= 0 && page < p.pages) atomicAdd(&p.refs[page], 1);
+    }
+    if (j == 0 && threadIdx.x == 0) {
+      if (to >= 0) p.table[d * p.width + full] = to;
+      p.lengths[d] = len;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kBlock) void k_free(tpi_pages p, const void* slots, int64_t n,
+                                                 bool wide) {
+  __shared__ int s_bad, s_len, s_count;
+  if (threadIdx.x == 0) {
+    s_bad = 0;
+    s_count = 0;
+  }
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < n; i += kBlock) {  // every workgroup comes to the same end
+    const int64_t s = number(slots, i, wide);
+    if (s < 0 || s >= p.slots) s_bad = 1;
+  }
+  __syncthreads();
+  if (s_bad) {
+    if (threadIdx.x == 0) refuse(p, TPI_PAGES_ESLOT);
+    return;
+  }
+  const int64_t s = number(slots, blockIdx.x, wide);
+  if (threadIdx.x == 0) s_len = atomicExch(&p.lengths[s], 0);  // named twice: empty by then
+  __syncthreads();
+  int32_t held = pages_of(s_len, p.tokens);
+  if (held > p.width) held = p.width;
+  for (int32_t k = threadIdx.x; k < held; k += kBlock) {
+    const int32_t page = p.table[s * p.width + k];
+    p.table[s * p.width + k] = -1;
+    if (page < 0 || page >= p.pages) continue;
+    if (atomicSub(&p.refs[page], 1) == 1) {
+      const uint32_t bit = 1u << (page & 31);
+      atomicOr(&p.free_bits[page >> 5], bit);
+      atomicOr(&p.stale_bits[page >> 5], bit);
+      atomicAdd(&s_count, 1);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && s_count) atomicAdd(&p.header[TPI_PAGES_FREE], s_count);
+}
+
+// Bits of word w whose page is below `page`.
+__device__ static inline uint32_t bits_below(int w, int page) {
+  const int64_t n = (int64_t)page - 32ll * w;
+  return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+}
+
+__global__ __launch_bounds__(kPlan) void k_plan(tpi_pages p, bool clear) {
+  const int tid = threadIdx.x;
+  const int live = p.pages - p.header[TPI_PAGES_FREE];
+  const int words = (p.pages + 31) / 32;
+  int holes = 0, movers = 0;
+  for (int base = 0; base < words; base += kPlan) {
+    int sum;
+    const int w = base + tid;
+    const uint32_t free = w < words ? p.free_bits[w] : 0;
+    const uint32_t low = bits_below(w, live), all = bits_below(w, p.pages);
+    const uint32_t hole = free & low, mover = ~free & all & ~low;
+    const int h = scan(__popc(hole), &sum);
+    emit(hole, w, holes + h, p.pages, list(p, HOLES));
+    holes += sum;
+    const int m = scan(__popc(mover), &sum);
+    emit(mover, w, movers + m, p.pages, list(p, MOVERS));
+    movers += sum;
+  }
+  __syncthreads();
+  // as many holes below `live` as live pages at or above it, if the counts are in order
+  const int moves = holes < movers ? holes : movers;
+  for (int i = tid; i < moves; i += kPlan) {
+    const int32_t from = list(p, MOVERS)[i], to = list(p, HOLES)[i];
+    p.refs[to] = p.refs[from];
+    p.refs[from] = 0;
+    list(p, MAP)[from] = to;
+  }
+  int clears = 0;
+  for (int base = 0; base < words; base += kPlan) {
+    int sum;
+    const int w = base + tid;
+    uint32_t stale = 0;
+    if (w < words) {
+      const uint32_t freed = bits_below(w, p.pages) & ~bits_below(w, live);
+      stale = (p.stale_bits[w] | ~p.free_bits[w]) & freed;  // a mover's old page is stale
+      p.free_bits[w] = freed;
+      p.stale_bits[w] = clear ? 0 : stale;
+    }
+    if (!clear) continue;
+    const int c = scan(__popc(stale), &sum);
+    emit(stale, w, clears + c, p.pages, list(p, CLEARS));
+    clears += sum;
+  }
+  if (tid == 0) {
+    p.header[TPI_PAGES_LIVE] = live;
+    p.header[TPI_PAGES_MOVES] = moves;
+    p.header[TPI_PAGES_CLEARS] = clears;
+  }
+}
+
+// The first `spans` workgroups take the table, the others the moved pages.
+__global__ __launch_bounds__(kBlock) void k_compact(tpi_pages p, int spans) {
+  const int live = p.header[TPI_PAGES_LIVE];
+  if ((int)blockIdx.x < spans) {
+    const int64_t entries = (int64_t)p.slots * p.width;
+    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < entries;
+         e += (int64_t)spans * kBlock) {
+      const int32_t page = p.table[e];
+      if (page >= live && page < p.pages) p.table[e] = list(p, MAP)[page];
+    }
+    return;
+  }
+  const int64_t work = (int64_t)p.header[TPI_PAGES_MOVES] * p.chunks;
+  for (int64_t w = blockIdx.x - spans; w < work; w += gridDim.x - spans) {
+    const int64_t i = w / p.chunks;
+    copy_chunk(p, (uint32_t)(w - i * p.chunks), list(p, MOVERS)[i], list(p, HOLES)[i]);
+  }
+}
+
+__global__ __launch_bounds__(kBlock) void k_clear(tpi_pages p) {
+  const int64_t work = (int64_t)p.header[TPI_PAGES_CLEARS] * p.chunks;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int64_t i = w / p.chunks;
+    zero_chunk(p, (uint32_t)(w - i * p.chunks), list(p, CLEARS)[i]);
+  }
+}
+
+constexpr int64_t kMaxGrid = 1 << 20;  // the loops over work take what a grid leaves
+constexpr int kSpread = 256 * 8;       // workgroups that fill the GPU
+
+uint32_t grid_of(int64_t work) { return (uint32_t)(work < kMaxGrid ? work : kMaxGrid); }
+
+}  // namespace
+
+extern "C" {
+
+int tpi_pages_copy(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
+                   uint64_t stream) {
+  if (n <= 0) return 0;
+  k_copy<<<grid_of(n * p->chunks), kBlock, 0, (hipStream_t)stream>>>(*p, src, dst, n, wide & 1);
+  TPI_HIP(hipGetLastError());
+  return 0;
+}
+
+int tpi_pages_fork(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
+                   uint64_t stream) {
+  if (n <= 0) return 0;
+  if (n > p->slots) return tpi_fail("fork: more destinations than slots");
+  hipStream_t s = (hipStream_t)stream;
+  k_reserve<true><<<1, kPlan, 0, s>>>(*p, src, dst, (int)n, wide & 1, nullptr, false, 0);
+  TPI_HIP(hipGetLastError());
+  const int spans = (p->width + kRowSpan - 1) / kRowSpan;
+  k_fork<<<grid_of(n * (spans + p->chunks)), kBlock, 0, s>>>(*p, src, dst, n, wide & 1, spans);
+  TPI_HIP(hipGetLastError());
+  return 0;
+}
+
+int tpi_pages_extend(const tpi_pages* p, const void* slots, int64_t n, int wide,
+                     const void* more, int64_t each, uint64_t stream) {
+  if (n <= 0) return 0;
+  if (n > p->slots) return tpi_fail("extend: more sequences than slots");
+  k_reserve<false><<<1, kPlan, 0, (hipStream_t)stream>>>(*p, slots, nullptr, (int)n, wide & 1,
+                                                         more, (wide & 2) != 0, each);
+  TPI_HIP(hipGetLastError());
+  return 0;
+}
+
+int tpi_pages_free(const tpi_pages* p, const void* slots, int64_t n, int wide, uint64_t stream) {
+  if (n <= 0) return 0;
+  if (n > p->slots) return tpi_fail("free: more sequences than slots");
+  k_free<<<(uint32_t)n, kBlock, 0, (hipStream_t)stream>>>(*p, slots, n, wide & 1);
+  TPI_HIP(hipGetLastError());
+  return 0;
+}
+
+int tpi_pages_compact(const tpi_pages* p, int clear, uint64_t stream) {
+  hipStream_t s = (hipStream_t)stream;
+  k_plan<<<1, kPlan, 0, s>>>(*p, clear != 0);
+  TPI_HIP(hipGetLastError());
+  const int64_t entries = (int64_t)p->slots * p->width;
+  const int spans = (int)(entries < 256ll * 1024 ? (entries + 1023) / 1024 : 256);
+  k_compact<<<spans + kSpread, kBlock, 0, s>>>(*p, spans);
+  TPI_HIP(hipGetLastError());
+  if (clear) {
+    k_clear<<<kSpread, kBlock, 0, s>>>(*p);
+    TPI_HIP(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // extern "C"

@@ -57,7 +57,7 @@ typedef struct tpi_stats {
 } tpi_stats;
 
 // Bumped whenever a signature below changes (ops/_loader.py checks it).
-#define TPI_ABI_VERSION 7
+#define TPI_ABI_VERSION 8
 
 // Library / device
 const char* tpi_last_error(void);
@@ -147,6 +147,88 @@ int tpi_pack_device(const tpi_seg* segs, const tpi_seg* host_segs, int n, uint64
 int tpi_unpack_device(const tpi_seg* segs, const tpi_seg* host_segs, int n, uint64_t total,
                       void* dev_src, uint64_t tile_bytes, const uint32_t* dev_crcs,
                       uint64_t* dev_bad, uint64_t stream);
+
+// ---- Dropout from a counter-based generator (ops/masking.py; csrc/common/philox.h) ------------
+enum { TPI_F32 = 0, TPI_F16 = 1, TPI_BF16 = 2 };
+// out = (kept ? x * scale : 0) + residual over a view of `ndim` dimensions (1 ..
+// TPI_MAX_DIMS, none empty, strides in elements).  `residual` (may be 0) has the output's
+// type.  Element i has index `first + sum(i[d] * si[d])` in the whole tensor.
+typedef struct tpi_dropout_args {
+  uint64_t x, residual, out;  // addresses: device memory for tpi_dropout
+  uint64_t state;             // {seed, draw} in device memory, read when the kernel runs and
+                              // `draw` below added to its second word; 0: `seed`, `draw`
+  uint64_t used;              // receives the {seed, draw} that was used; may be 0
+  uint64_t seed, draw;        // draw < 2^63
+  uint64_t first;
+  uint64_t threshold;         // share kept * 2^32, 0 .. 2^32
+  int64_t sizes[TPI_MAX_DIMS], sx[TPI_MAX_DIMS], sr[TPI_MAX_DIMS], so[TPI_MAX_DIMS],
+      si[TPI_MAX_DIMS];
+  float scale;
+  int32_t in_type, out_type;  // TPI_F32 .. TPI_BF16: equal, or one of them TPI_F32
+  int32_t ndim;
+} tpi_dropout_args;
+int tpi_dropout(const tpi_dropout_args* args, uint64_t stream);
+
+// ---- Pages of a paged cache (ops/paging.py) ----------------------------------------------------
+// One tensor whose first dimension is the page: `rows` runs of `row_bytes` bytes per page.
+// Pages are moved in chunks of TPI_PAGE_UNITS units of `unit` bytes (16, 8, 4, 2 or 1: what
+// base, strides and row_bytes are multiples of); chunk0 = chunks of the tensors before it.
+#define TPI_PAGE_UNITS 1024
+typedef struct tpi_page_tensor {
+  uint64_t base;
+  int64_t page_stride, row_stride;  // bytes
+  uint32_t rows, row_units, unit, chunk0;
+} tpi_page_tensor;
+enum {  // words of the header
+  TPI_PAGES_FREE = 0,    // pages without a reference
+  TPI_PAGES_ERROR = 1,   // first refusal since it was last cleared, TPI_PAGES_E*
+  TPI_PAGES_LIVE = 2,    // scratch of a compaction: live pages, pages to move, pages to clear
+  TPI_PAGES_MOVES = 3,
+  TPI_PAGES_CLEARS = 4,
+  TPI_PAGES_HEADER = 16
+};
+enum {
+  TPI_PAGES_ENOSPACE = 1,    // not enough free pages
+  TPI_PAGES_ESLOT = 2,       // a slot out of range
+  TPI_PAGES_EBUSY = 3,       // fork into a slot that holds a sequence
+  TPI_PAGES_EWIDTH = 4,      // a sequence longer than a row of the table
+  TPI_PAGES_EPAGE = 5,       // a page out of range
+  TPI_PAGES_EDUPLICATE = 6,  // a slot named twice
+  TPI_PAGES_ETOKENS = 7,     // a negative number of tokens
+  TPI_PAGES_ESTATE = 8,      // the bookkeeping contradicts itself
+};
+// A pool's state; every address is device memory (host memory for the host implementation).
+typedef struct tpi_pages {
+  int32_t* header;
+  int32_t* refs;         // [pages] table entries that name the page
+  int32_t* lengths;      // [slots] tokens of the slot's sequence
+  int32_t* table;        // [slots][width] pages of the sequence, -1 behind its end
+  uint32_t* free_bits;   // [ceil(pages / 32)] 1: no reference
+  uint32_t* stale_bits;  // [ceil(pages / 32)] 1: not known to be zero (free pages only)
+  int32_t* scratch;      // 4 * pages + 5 * slots words
+  const tpi_page_tensor* tensors;
+  int32_t pages, slots, width, tokens;
+  int32_t ntensors;
+  int32_t chunks;        // of one page, over all tensors
+} tpi_pages;
+// `wide` bit 0: slot / page numbers are int64, else int32; bit 1: the same of `more`.
+// copy: page src[i] to page dst[i] in every tensor; no page may be a destination twice, nor a
+// destination and a source.  A pair with a number out of range is left out (EPAGE).
+int tpi_pages_copy(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
+                   uint64_t stream);
+// The next four change nothing when they refuse (the reason goes to the header); n <= slots.
+// fork: slot dst[i] becomes a copy of slot src[i]: full pages shared, a partial last page copied.
+int tpi_pages_fork(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
+                   uint64_t stream);
+// extend: slot slots[i] grows by more[i] tokens (more == NULL: by `each`), lowest free pages
+// first.
+int tpi_pages_extend(const tpi_pages* p, const void* slots, int64_t n, int wide,
+                     const void* more, int64_t each, uint64_t stream);
+// free: the slots become empty; a slot named twice is freed once.
+int tpi_pages_free(const tpi_pages* p, const void* slots, int64_t n, int wide, uint64_t stream);
+// compact: the live pages become pages 0 .. live - 1 (the i-th hole below takes the i-th live
+// page above); `clear`: free pages that are not known to be zero are cleared.
+int tpi_pages_compact(const tpi_pages* p, int clear, uint64_t stream);
 
 // Host memory: NUMA-bound, populated, registered (pinned) mappings.
 // path == NULL -> anonymous; otherwise a shared file (e.g. /dev/shm/...) that outlives the

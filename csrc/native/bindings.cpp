@@ -2,6 +2,8 @@
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
+#include <string.h>
+
 #include <stdexcept>
 
 #include "ctl.h"
@@ -9,6 +11,7 @@
 #include "../common/tpz.h"
 #include "fileio.h"
 #include "hostops.h"
+#include "stateops.h"
 #include "transfer.h"
 
 namespace py = pybind11;
@@ -21,6 +24,15 @@ const tpi_seg* seg_ptr(py::buffer& b, int& n) {
     throw std::invalid_argument("segment buffer size is not a multiple of sizeof(tpi_seg)");
   n = (int)(info.size * info.itemsize / sizeof(tpi_seg));
   return (const tpi_seg*)info.ptr;
+}
+
+template <typename T>
+T struct_of(const py::bytes& b) {  // a C struct laid out by the caller
+  const std::string raw = b;
+  if (raw.size() != sizeof(T)) throw std::invalid_argument("argument block has a wrong size");
+  T out;
+  memcpy(&out, raw.data(), sizeof(T));
+  return out;
 }
 
 }  // namespace
@@ -165,6 +177,29 @@ PYBIND11_MODULE(_tpi_native, m) {
                         &first);
     }
     return py::make_tuple(bad, first);
+  });
+  m.attr("DROPOUT_ARGS_SIZE") = (int)sizeof(tpi_dropout_args);
+  m.attr("PAGES_SIZE") = (int)sizeof(tpi_pages);
+  m.attr("PAGE_TENSOR_SIZE") = (int)sizeof(tpi_page_tensor);
+  m.def("dropout", [](const py::bytes& args, int threads) {
+    const tpi_dropout_args a = struct_of<tpi_dropout_args>(args);
+    py::gil_scoped_release nogil;
+    tpi::dropout(a, threads);
+  });
+  m.def("pages_copy", [](const py::bytes& pool, uintptr_t src, uintptr_t dst, int64_t n) {
+    tpi::pages_copy(struct_of<tpi_pages>(pool), (const int64_t*)src, (const int64_t*)dst, n);
+  });
+  m.def("pages_fork", [](const py::bytes& pool, uintptr_t src, uintptr_t dst, int64_t n) {
+    tpi::pages_fork(struct_of<tpi_pages>(pool), (const int64_t*)src, (const int64_t*)dst, n);
+  });
+  m.def("pages_extend", [](const py::bytes& pool, uintptr_t slots, uintptr_t more, int64_t n) {
+    tpi::pages_extend(struct_of<tpi_pages>(pool), (const int64_t*)slots, (const int64_t*)more, n);
+  });
+  m.def("pages_free", [](const py::bytes& pool, uintptr_t slots, int64_t n) {
+    tpi::pages_free(struct_of<tpi_pages>(pool), (const int64_t*)slots, n);
+  });
+  m.def("pages_compact", [](const py::bytes& pool, bool clear) {
+    tpi::pages_compact(struct_of<tpi_pages>(pool), clear);
   });
   m.def("write_file_ptr", [](const std::string& path, uintptr_t src, uint64_t n, int threads,
                             bool sync) {

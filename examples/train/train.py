@@ -39,6 +39,9 @@ def main():
     p.add_argument("--sleep", type=float, default=0.0, help="sleep per step (tests)")
     p.add_argument("--ckpt-every", type=int, default=0,
                    help="asynchronous checkpoint every N steps (0: only on SIGTERM/exit)")
+    p.add_argument("--dropout", type=float, default=0.0,
+                   help="drop this share of each block's output; its masks come from a counter "
+                        "in the checkpoint, so a resumed run draws the same")
     p.add_argument("--materialize", action="store_true",
                    help="resume by materializing the state from the spill (the model is built "
                         "on the meta device; for ranks bigger than half of HBM; one rank)")
@@ -96,12 +99,19 @@ def main():
 
     torch.manual_seed(1234)
     h = args.hidden
+    stateful = {}
+    if args.dropout:
+        from terraform_provider_iterative_amd import ops
+
+        stateful["masks"] = masks = ops.MaskStream(seed=1234 + rank)  # each rank's batch its own
 
     def build():
         layers = []
         for _ in range(args.layers):
             layers += [torch.nn.LayerNorm(h), torch.nn.Linear(h, 4 * h), torch.nn.GELU(),
                        torch.nn.Linear(4 * h, h)]
+            if args.dropout:
+                layers.append(ops.CounterDropout(args.dropout, masks))
         return torch.nn.Sequential(*layers)
 
     def make_opt(m):
@@ -116,7 +126,8 @@ def main():
         # allocation of a model that would not fit next to the predecessor's
         with torch.device("meta"):
             model = build().to(torch.bfloat16)
-        state = TrainingState.from_materialized(got, model, make_opt, generators={"data": gen})
+        state = TrainingState.from_materialized(got, model, make_opt, generators={"data": gen},
+                                                stateful=stateful)
         opt, step_t, meta = state.optimizer, got[1]["extra.step"], got[2]
     else:
         model = build().to(device=device, dtype=torch.bfloat16)
@@ -132,7 +143,7 @@ def main():
         # model + optimizer device state by reference; CPU-side Adam step counters, the
         # optimizer hyper-parameters, every RNG and `gen` ride in the checkpoint header
         state = TrainingState(model, opt, extra={"step": step_t}, path=spill,
-                              generators={"data": gen})
+                              generators={"data": gen}, stateful=stateful)
         # ranks agree on the step to resume from (or all start fresh)
         meta = state.resume_consistent() if world > 1 else state.resume()
     ck = state.checkpointer

@@ -62,6 +62,7 @@ _note_lock = threading.Lock()
 _signal_info: Dict[str, float] = {}
 _boundary_seen = False           # the loop calls step()/tick(): saves wait for a boundary
 _last_step: Optional[int] = None  # user step of the last boundary
+_mid_step = False                # a torn-risk / signal-time save has begun
 _agreement = None
 _wakeup_r: Optional[int] = None
 _standby_script = False          # the script calls standby(spill): its successor waits for HBM
@@ -85,6 +86,12 @@ def preempted() -> bool:
 
 def saving() -> bool:
     return _fired.is_set()
+
+
+def mid_step() -> bool:
+    """The save that is running was forced between two step boundaries: callbacks must leave the
+    registered tensors' content alone, the step's own work may still be using it."""
+    return _mid_step
 
 
 def journal(code: str, *description: str) -> None:
@@ -657,9 +664,10 @@ def _save_and_exit(consistency: str, ordinal: Optional[int] = None) -> None:
     * a failed spill after an HBM export still waits for the successor: its device copy is
       then the only good one.
     """
-    global _handoff_decision
+    global _handoff_decision, _mid_step
     if not _save_lock.acquire(blocking=False):
         return
+    _mid_step = consistency != "boundary"
     _fired.set()
     signum = int(_signal_info.get("signum", signal.SIGTERM))
     t0 = time.perf_counter()

@@ -13,7 +13,9 @@ initialised GPU, Python ``random``, NumPy's global generator, plus any ``generat
 in), the optimizer's hyper-parameters per param group (an LR schedule changes them), the LR
 scheduler, the AMP ``GradScaler``, and any object with ``state_dict``/``load_state_dict``
 registered as ``stateful`` (a sampler, a data cursor: :class:`DataCursor`).  All of it is
-captured at the same step boundary as the tensors.
+captured at the same step boundary as the tensors.  Draws of :func:`..ops.dropout` are numbered
+by a ``MaskStream`` (``stateful``); the pages of a paged cache (``paged``, :class:`..ops.PagePool`)
+are checkpointed with its books, compacted first.
 
 This is the tensor-level counterpart of the reference's workdir sync: there the user script
 had to re-read its own files after a spot respawn (README.md:93-101).
@@ -32,8 +34,10 @@ HOST_NUMEL_LIMIT = 4096  # per host tensor carried in the JSON header
 
 
 def collect(model, optimizer=None, extra: Optional[Dict[str, Any]] = None,
-            device=None) -> Tuple[Dict[str, Any], Dict[str, Any]]:
-    """(tensors on ``device``, small tensors elsewhere) of a model/optimizer pair.
+            device=None, paged: Optional[Dict[str, Any]] = None
+            ) -> Tuple[Dict[str, Any], Dict[str, Any]]:
+    """(tensors on ``device``, small tensors elsewhere) of a model/optimizer pair and of
+    ``paged`` pools.
 
     ``device`` defaults to the device of the model's first parameter.  Optimizer state needs
     to exist (take one step first: PyTorch creates it lazily).
@@ -69,6 +73,13 @@ def collect(model, optimizer=None, extra: Optional[Dict[str, Any]] = None,
                 put("optim.%d.%s" % (i, key), value)
     for name, t in (extra or {}).items():
         put("extra." + name, t)
+    for name, pool in (paged or {}).items():
+        if pool.meta.device != device:
+            raise ValueError("paged %r is on %s, the checkpoint on %s" % (name, pool.meta.device,
+                                                                         device))
+        put("paged.%s.meta" % name, pool.meta)
+        for i, t in enumerate(pool.tensors):
+            put("paged.%s.%d" % (name, i), t)
     return main, host
 
 
@@ -251,14 +262,22 @@ class TrainingState:
     whatever else makes up the step): that is where a preemption is saved -- on every rank at
     the same boundary -- and where periodic checkpoints are taken.  Every save records the step
     number in its metadata (``"step"``), so :meth:`resume_consistent` compares real steps.
+
+    ``paged={"kv": pool}``: the tensors and books of paged caches (:class:`..ops.PagePool`).  A save
+    at a boundary first moves a pool's live pages together and clears the dead ones, so that the
+    codec spills live pages only; page numbers are the table's from then on (a save in the middle
+    of a step leaves the pages where they are).  Pools have to be on the checkpoint's device, and
+    are resumed with :meth:`resume` (not :meth:`from_materialized`).
     """
 
     def __init__(self, model, optimizer=None, extra: Optional[Dict[str, Any]] = None,
                  path: Optional[str] = None, device=None, *, lr_scheduler=None, scaler=None,
                  rng: bool = True, generators: Optional[Dict[str, Any]] = None,
                  stateful: Optional[Dict[str, Any]] = None,
+                 paged: Optional[Dict[str, Any]] = None,
                  checkpointer: Optional[Checkpointer] = None, **checkpointer_kwargs):
-        tensors, self.host = collect(model, optimizer, extra, device)
+        self.paged: Dict[str, Any] = dict(paged or {})
+        tensors, self.host = collect(model, optimizer, extra, device, self.paged)
         if not tensors:
             raise ValueError("nothing to checkpoint on the model's device")
         self.optimizer = optimizer
@@ -303,6 +322,8 @@ class TrainingState:
         import torch
 
         ck, tensors, meta = materialized
+        if any(k.startswith("paged.") for k in tensors):
+            raise ValueError("the checkpoint has paged caches: resume() into their pools instead")
         blobs = (meta or {}).get("host_tensors", {})
 
         def host_tensor(name):
@@ -370,6 +391,9 @@ class TrainingState:
                 "training_state": state}
 
     def _metadata(self, metadata: Optional[Dict] = None) -> Dict[str, Any]:
+        if not preemption.mid_step():  # between steps nothing else touches the pages
+            for pool in self.paged.values():
+                pool.compact(clear=True)
         meta: Dict[str, Any] = {}
         if self.step_value is not None:
             meta["step"] = self.step_value

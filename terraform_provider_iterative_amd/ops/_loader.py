@@ -14,7 +14,7 @@ from typing import Optional
 
 from .. import _build
 
-ABI_VERSION = 7  # TPI_ABI_VERSION of csrc/hip/tpi_hip.h
+ABI_VERSION = 8  # TPI_ABI_VERSION of csrc/hip/tpi_hip.h
 
 _lock = threading.Lock()
 _native = None
@@ -123,6 +123,12 @@ class HipLib:
             "tpi_shard_hash": (i32, [vp, u64, u64, u64, vp, u64]),
             "tpi_pack_device": (i32, [vp, vp, i32, u64, vp, u64, vp, u64]),
             "tpi_unpack_device": (i32, [vp, vp, i32, u64, vp, u64, vp, vp, u64]),
+            "tpi_dropout": (i32, [c.c_char_p, u64]),
+            "tpi_pages_copy": (i32, [c.c_char_p, vp, vp, i64, i32, u64]),
+            "tpi_pages_fork": (i32, [c.c_char_p, vp, vp, i64, i32, u64]),
+            "tpi_pages_extend": (i32, [c.c_char_p, vp, i64, i32, vp, i64, u64]),
+            "tpi_pages_free": (i32, [c.c_char_p, vp, i64, i32, u64]),
+            "tpi_pages_compact": (i32, [c.c_char_p, i32, u64]),
             "tpi_host_map": (vp, [c.c_char_p, u64, i32, i32]),
             "tpi_host_unmap": (i32, [vp, u64]),
             "tpi_host_register": (i32, [vp, u64]),

@@ -1,0 +1,307 @@
+"""Dropout from a counter-based generator; its mask is never stored.
+
+Whether an element is kept depends on three things only: a seed, the number of the draw, and the
+element's index in the whole tensor (the definition is in ``csrc/common/philox.h``).  So
+
+* the backward pass draws the mask again instead of reading it back,
+* a checkpoint carries two integers (:class:`MaskStream` is ``stateful`` for
+  :class:`~..checkpoint.TrainingState`), and a resumed rank draws what the uninterrupted one
+  would have,
+* the masks do not depend on how many ranks share a tensor (``shard=``): a gang that resumes
+  with another number of ranks goes on with the same masks.
+
+Device tensors go through ``csrc/hip/dropout.hip``, host tensors through
+``csrc/native/stateops.cpp``; both give the same bits.
+"""
+from __future__ import annotations
+
+import struct
+from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
+
+import torch
+
+from ._loader import hip, native
+from .packing import MAX_DIMS
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # TPI_F32 .. TPI_BF16
+_ARGS = struct.Struct("<9Q%dqf3i" % (5 * MAX_DIMS))  # tpi_dropout_args
+_WHOLE = 1 << 32
+_PAD = (0,) * MAX_DIMS
+
+
+class Draw(NamedTuple):
+    """What names one mask: ``(seed, number)``, or with ``state`` (an int64 tensor ``[seed,
+    number]`` on the operand's device) ``state``'s seed and ``number`` past ``state``'s."""
+    seed: int
+    number: int
+    state: Optional[torch.Tensor] = None
+
+
+class MaskStream:
+    """Hands out draw numbers, and is what a checkpoint carries of all masks::
+
+        masks = MaskStream(seed=7)
+        state = TrainingState(model, opt, path=spill, stateful={"masks": masks})
+        y = dropout(x, 0.1, masks)
+
+    Each :func:`dropout` given the stream takes the next number.  A block that is computed twice
+    (activation checkpointing) has to draw the same mask both times: take ``masks.next()``
+    outside it and pass that.
+
+    With ``device`` the seed and number are held there and read when a kernel runs, so that a
+    captured graph draws new masks at every replay: call :meth:`advance` once per step, inside
+    the capture, after the step's last draw.  Without it a capture is refused, because every
+    replay would repeat the captured masks.
+    """
+
+    def __init__(self, seed: int = 0, number: int = 0, device=None):
+        _check_key(seed, number)
+        self.seed, self.number = int(seed), int(number)
+        self.state: Optional[torch.Tensor] = None
+        if device is not None:
+            self.state = torch.tensor([_signed(self.seed), self.number], dtype=torch.int64,
+                                      device=device)
+            self._ahead = 0
+
+    def next(self) -> Draw:
+        if self.state is not None:
+            self._ahead += 1
+            return Draw(0, self._ahead - 1, self.state)
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise ValueError("a captured graph would repeat this stream's masks at every replay: "
+                             "give MaskStream a device")
+        self.number += 1
+        return Draw(self.seed, self.number - 1)
+
+    def advance(self) -> None:
+        """End of a step (device streams): the next step's draws come after this one's."""
+        if self.state is None:
+            raise ValueError("advance() is for a MaskStream with a device")
+        self.state[1:].add_(self._ahead)
+        self._ahead = 0
+
+    def state_dict(self) -> dict:
+        seed, number = self.seed, self.number
+        if self.state is not None:
+            seed, number = self.state.tolist()
+            seed, number = seed % (1 << 64), number + self._ahead
+        return {"seed": seed, "number": number}
+
+    def load_state_dict(self, state: dict) -> None:
+        seed, number = int(state["seed"]), int(state["number"])
+        _check_key(seed, number)
+        if self.state is not None:
+            self.state.copy_(torch.tensor([_signed(seed), number], dtype=torch.int64))
+            self._ahead = 0
+        else:
+            self.seed, self.number = seed, number
+
+
+def _signed(value: int) -> int:
+    return value - (1 << 64) if value >> 63 else value
+
+
+def _check_key(seed, number) -> None:
+    if not 0 <= seed < 1 << 64:
+        raise ValueError("seed must be in [0, 2^64)")
+    if not 0 <= number < 1 << 63:
+        raise ValueError("draw number must be in [0, 2^63)")
+
+
+def _as_draw(draw) -> Draw:
+    if isinstance(draw, MaskStream):
+        return draw.next()
+    if not isinstance(draw, Draw):
+        try:
+            seed, number = draw
+        except (TypeError, ValueError):
+            raise TypeError("draw must be a MaskStream, a Draw or (seed, number)") from None
+        draw = Draw(int(seed), int(number))
+    _check_key(draw.seed, draw.number)
+    if draw.state is not None and (draw.state.dtype != torch.int64 or draw.state.numel() != 2
+                                   or not draw.state.is_contiguous()):
+        raise ValueError("a draw's state must be two contiguous int64")
+    return draw
+
+
+def keep_threshold(p: float) -> Tuple[int, float]:
+    """``(threshold, scale)`` of a drop probability: an element is kept when its 32-bit uniform
+    number is below ``threshold``, and the scale is the inverse of the share that this keeps
+    (``threshold / 2^32``), not of ``1 - p``, so that the expectation is exact."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:  # NaN too
+        raise ValueError("dropout probability must be in [0, 1]")
+    threshold = int(round((1.0 - p) * _WHOLE))
+    return threshold, (_WHOLE / threshold if threshold else 0.0)
+
+
+def _merged(shape: Sequence[int], *strides: Sequence[int]) -> List[Tuple[int, ...]]:
+    """``(size, stride of each operand)`` dims, size-1 dims dropped and dims merged that every
+    operand walks as one."""
+    dims: List[Tuple[int, ...]] = []
+    for dim in zip(shape, *strides):
+        size = dim[0]
+        if size == 1:
+            continue
+        if dims and all(a == b * size for a, b in zip(dims[-1][1:], dim[1:])):
+            dims[-1] = (dims[-1][0] * size,) + dim[1:]
+        else:
+            dims.append(dim)
+    return dims or [(1,) * (1 + len(strides))]
+
+
+class _Plan(NamedTuple):
+    threshold: int
+    scale: float
+    first: int                            # index of the view's first element in the whole tensor
+    strides: Optional[Tuple[int, ...]]    # index strides, None: the view is the whole tensor
+
+
+def _shard_plan(shape, shard) -> Tuple[int, Optional[Tuple[int, ...]]]:
+    if shard is None:
+        return 0, None
+    whole, starts = (tuple(int(v) for v in part) for part in shard)
+    if len(whole) != len(shape) or len(starts) != len(shape):
+        raise ValueError("shard must give a size and a start for each of the %d dimensions"
+                         % len(shape))
+    strides, step, first = [], 1, 0
+    for size, lo, n in zip(reversed(whole), reversed(starts), reversed(shape)):
+        if lo < 0 or lo + n > size:
+            raise ValueError("shard %s at %s is not inside %s" % (tuple(shape), starts, whole))
+        strides.append(step)
+        first += lo * step
+        step *= size
+    if step >= 1 << 63:
+        raise ValueError("the whole tensor is too large")
+    return first, tuple(reversed(strides))
+
+
+def _contiguous_strides(shape) -> Tuple[int, ...]:
+    out, step = [], 1
+    for size in reversed(shape):
+        out.append(step)
+        step *= size
+    return tuple(reversed(out))
+
+
+def _apply(x, residual, out_dtype, plan: _Plan, draw: Draw, used=None):
+    """One pass: ``(kept ? x * scale : 0) + residual`` in ``out_dtype``."""
+    out = torch.empty_like(x if residual is None else residual, dtype=out_dtype)
+    if x.numel() == 0:  # nor will the backward pass read `used`
+        return out
+    if plan.strides is None and x.is_contiguous() and out.is_contiguous() and (
+            residual is None or residual.is_contiguous()):
+        n = x.numel()
+        ndim, sizes, ones = 1, (n,) + _PAD[1:], (1,) + _PAD[1:]
+        walk = sizes + ones * 4
+    else:
+        index = plan.strides if plan.strides is not None else _contiguous_strides(x.shape)
+        operands = [x.stride(), out.stride() if residual is None else residual.stride(),
+                    out.stride(), index]
+        dims = _merged(x.shape, *operands)
+        ndim = len(dims)
+        if ndim > MAX_DIMS:
+            raise ValueError("tensors with more than %d (merged) dims are not supported" % MAX_DIMS)
+        walk = ()
+        for column in zip(*dims):
+            walk += tuple(column) + _PAD[ndim:]
+    state, seed = draw.state, draw.seed
+    args = _ARGS.pack(x.data_ptr(), 0 if residual is None else residual.data_ptr(),
+                      out.data_ptr(), 0 if state is None else state.data_ptr(),
+                      0 if used is None else used.data_ptr(), seed, draw.number, plan.first,
+                      plan.threshold, *walk, plan.scale, _TYPES[x.dtype], _TYPES[out_dtype], ndim)
+    if x.device.type == "cuda":
+        lib = hip()
+        with torch.cuda.device(x.device):
+            lib.check(lib.tpi_dropout(args, torch.cuda.current_stream().cuda_stream), "dropout")
+    else:
+        native().dropout(args, torch.get_num_threads())
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    """The gradient of a dropped element is 0, of a kept one the scale times the output's: the
+    operator itself, applied to the gradient (so it can be differentiated again)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, out_dtype, plan, draw):
+        ctx.plan, ctx.draw, ctx.x_dtype = plan, draw, x.dtype
+        used = None
+        if draw.state is not None and ctx.needs_input_grad[0]:
+            # the state may have moved on by the time the backward pass runs
+            used = torch.empty(2, dtype=torch.int64, device=x.device)
+            ctx.draw = Draw(0, 0, used)
+        return _apply(x, residual, out_dtype, plan, draw, used)
+
+    @staticmethod
+    def backward(ctx, grad):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _run(grad, None, ctx.x_dtype, ctx.plan, ctx.draw)
+        return dx, grad if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def _run(x, residual, out_dtype, plan, draw):
+    if torch.is_grad_enabled() and (x.requires_grad or
+                                    (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, out_dtype, plan, draw)
+    return _apply(x, residual, out_dtype, plan, draw)
+
+
+def dropout(x: torch.Tensor, p: float, draw: Union[MaskStream, Draw, Tuple[int, int]], *,
+            residual: Optional[torch.Tensor] = None,
+            shard: Optional[Tuple[Sequence[int], Sequence[int]]] = None) -> torch.Tensor:
+    """``x`` with each element dropped with probability ``p`` and the others scaled by
+    ``1 / (1 - p)``, plus ``residual``; differentiable in both.
+
+    ``x`` is float32, float16 or bfloat16, on the GPU or the host, of any strides that merge into
+    6 dimensions.  ``residual`` has its shape and device, and its type or float32; the result
+    has the residual's type (computed in 32 bits, rounded once).  A dropped element contributes
+    0 whatever ``x`` holds there.  ``p`` is taken to the nearest multiple of 2^-32.
+
+    ``draw`` names the mask: a :class:`MaskStream` (its next number), or ``(seed, number)``,
+    which gives the same mask at every call (and every replay of a captured one).
+    ``shard=(whole_shape, starts)`` says that ``x`` is the block of a tensor of ``whole_shape``
+    that begins at ``starts``: it is masked as that block of the whole would be.
+
+    The result is enqueued on the current stream of ``x``'s device.
+    """
+    if not isinstance(x, torch.Tensor) or x.device.type not in ("cuda", "cpu"):
+        raise TypeError("dropout needs a tensor on the GPU or the host")
+    if x.dtype not in _TYPES:
+        raise TypeError("dropout of %s is not supported (float32, float16, bfloat16)" % x.dtype)
+    threshold, scale = keep_threshold(p)
+    out_dtype = x.dtype
+    if residual is not None:
+        if not isinstance(residual, torch.Tensor) or residual.device != x.device:
+            raise ValueError("the residual must be a tensor on %s" % x.device)
+        if residual.shape != x.shape:  # a broadcast one: expand it, its gradient is summed there
+            raise ValueError("the residual's shape %s is not x's %s (expand it first)"
+                             % (tuple(residual.shape), tuple(x.shape)))
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise TypeError("the residual must be %s or float32" % x.dtype)
+        out_dtype = residual.dtype
+    first, strides = _shard_plan(x.shape, shard)
+    draw = _as_draw(draw)
+    if draw.state is not None and draw.state.device != x.device:
+        raise ValueError("the mask stream is on %s, the tensor on %s" % (draw.state.device,
+                                                                         x.device))
+    return _run(x, residual, out_dtype, _Plan(threshold, scale, first, strides), draw)
+
+
+class CounterDropout(torch.nn.Module):
+    """:func:`dropout` as a layer: ``layer(x)`` or ``layer(x, residual)``.  Layers of a model
+    share one :class:`MaskStream`; in evaluation nothing is drawn or dropped."""
+
+    def __init__(self, p: float, stream: MaskStream):
+        super().__init__()
+        keep_threshold(p)
+        self.p, self.stream = float(p), stream
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.training:
+            return dropout(x, self.p, self.stream, residual=residual)
+        return x if residual is None else dropout(x, 0.0, (0, 0), residual=residual)
+
+    def extra_repr(self) -> str:
+        return "p=%g" % self.p

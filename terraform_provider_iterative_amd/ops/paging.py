@@ -1,0 +1,304 @@
+"""Pages of a paged cache: copying, forking, extending, freeing and compacting.
+
+A cache of many sequences is kept in pages of ``page_tokens`` tokens; page ``i`` is row ``i`` of
+each of a set of tensors (keys and values of every layer).  :class:`PagePool` keeps the books on
+the device beside it -- which pages a sequence has, how many sequences name a page, which pages
+are free -- and moves pages' bytes in all tensors with one launch.  No operation waits for the
+host, so they can be captured into a graph; the host reads the books when it asks
+(:meth:`PagePool.status`).
+
+Results are the same on every run and on the host (``csrc/hip/pages.hip``,
+``csrc/native/stateops.cpp``): free pages are taken lowest number first, in the order in which
+sequences are named.
+
+The books are one int32 tensor (:attr:`PagePool.meta`).  ``TrainingState(paged={"kv": pool})``
+checkpoints it with the pool's tensors, after the live pages have been moved together and the
+dead ones cleared: those cost a spill through the codec next to nothing.
+"""
+from __future__ import annotations
+
+import struct
+from typing import Any, Dict, List, Optional, Sequence, Union
+
+import numpy as np
+import torch
+
+from ._loader import hip, native
+from .packing import canonical_view
+
+HEADER, CHUNK_UNITS = 16, 1024  # TPI_PAGES_HEADER, TPI_PAGE_UNITS
+_POOL = struct.Struct("<8Q6i")  # tpi_pages
+_TENSOR = struct.Struct("<Q2q4I")  # tpi_page_tensor
+_FREE, _ERROR = 0, 1
+_ERRORS = {1: "not enough free pages", 2: "a slot is out of range",
+           3: "a fork's destination holds a sequence (or is its source)",
+           4: "a sequence would be longer than a row of the table",
+           5: "a page is out of range", 6: "a slot is named twice",
+           7: "a negative number of tokens", 8: "the pool's books contradict themselves"}
+
+Numbers = Union[Sequence[int], torch.Tensor]
+
+
+class PageError(RuntimeError):
+    """A pool refused an operation."""
+
+
+def _pad4(words: int) -> int:
+    return (words + 3) // 4 * 4
+
+
+class PagePool:
+    """The pages of ``tensors`` and the ``slots`` sequences that hold them.
+
+    ``tensors``: one or more tensors of one device whose first dimension is the page, all with the
+    same number of pages; a page's bytes are one contiguous run, or several with one stride
+    between them (``[heads, pages, ...]`` storage seen pages first).  ``page_tokens``: tokens
+    of a page.  ``width``: pages that one sequence can have (default: all).
+
+    * :attr:`table` ``[slots, width]`` int32: pages of each slot's sequence, -1 behind its end
+    * :attr:`lengths` ``[slots]`` int32: its tokens; 0: the slot is free
+    * :attr:`refs` ``[pages]`` int32: table entries that name the page; 0: the page is free
+
+    They are views of :attr:`meta` for kernels to read; change them through the methods (or
+    :meth:`bind`) only.  Operations are enqueued on the current stream of the pool's device; two
+    on one pool must not run at the same time, on two streams or in two graphs.  Slots and pages
+    are given as lists, or as int32 / int64 tensors on the pool's device, read when the kernel
+    runs.  An operation that cannot be done as a whole changes nothing: numbers given as lists
+    that are out of range or named twice raise ``ValueError`` at once; what only the device can
+    see (too few free pages, say) raises :class:`PageError` at the next :meth:`check`, on the host
+    at once.
+    """
+
+    def __init__(self, tensors: Sequence[torch.Tensor], page_tokens: int, slots: int,
+                 width: Optional[int] = None):
+        tensors = list(tensors)
+        if not tensors or not all(isinstance(t, torch.Tensor) for t in tensors):
+            raise ValueError("a pool needs at least one tensor")
+        self.device = tensors[0].device
+        if self.device.type not in ("cuda", "cpu"):
+            raise ValueError("a pool's tensors must be on the GPU or the host")
+        if any(t.dim() < 2 or t.numel() == 0 for t in tensors):
+            raise ValueError("a pool's tensors need a page dimension and bytes in each page")
+        if len({(t.device, t.shape[0]) for t in tensors}) != 1:
+            raise ValueError("a pool's tensors must be on one device, with as many pages each")
+        self.pages, self.page_tokens, self.slots = tensors[0].shape[0], int(page_tokens), int(slots)
+        self.width = self.pages if width is None else int(width)
+        if not 1 <= self.page_tokens <= 1 << 20:
+            raise ValueError("page_tokens must be in [1, 2^20]")
+        if self.slots < 1 or self.width < 1:
+            raise ValueError("slots and width must be positive")
+        # 32-bit numbers, and a prefix of every word that one scan of the kernels can add up
+        if self.pages >= 1 << 30 or self.slots >= 1 << 30 or self.width >= 1 << 30:
+            raise ValueError("too many pages, slots or pages of a sequence")
+        self.tensors = tensors
+        self._lay_out_tensors()
+        words = (self.pages + 31) // 32
+        sizes = [HEADER, _pad4(self.pages), _pad4(self.slots), _pad4(self.slots * self.width),
+                 _pad4(words), _pad4(words)]
+        self.meta = torch.zeros(sum(sizes), dtype=torch.int32, device=self.device)
+        self._bind_meta(sizes, words)
+        self._scratch = torch.empty(4 * self.pages + 5 * self.slots, dtype=torch.int32,
+                                    device=self.device)
+        at = [t.data_ptr() for t in (self._header, self.refs, self.lengths, self.table,
+                                     self._free_bits, self._stale_bits, self._scratch,
+                                     self._descriptors)]
+        self._args = _POOL.pack(*at, self.pages, self.slots, self.width, self.page_tokens,
+                                len(tensors), self._chunks)
+        self._write_books(np.full((self.slots, self.width), -1, np.int32),
+                          np.zeros(self.slots, np.int32))
+
+    def _lay_out_tensors(self) -> None:
+        rows, chunk0 = [], 0
+        for t in self.tensors:
+            elem = t.element_size()
+            strides = sorted((st, size) for st, size in zip(t.stride(), t.shape) if size > 1)
+            if any(st <= 0 or (i and st < strides[i - 1][0] * strides[i - 1][1])
+                   for i, (st, _) in enumerate(strides)):
+                raise ValueError("a pool's tensors must not overlap themselves")
+            dims = canonical_view(t.shape[1:], t.stride()[1:])
+            if dims[-1][1] != 1:  # elements with gaps between them: runs of one element
+                dims.append((1, 1))
+            if len(dims) > 2:
+                raise ValueError("a page's bytes must be contiguous runs with one stride between "
+                                 "them, not %s with strides %s" % (tuple(t.shape), t.stride()))
+            runs, run_stride = dims[0] if len(dims) == 2 else (1, 0)
+            run = dims[-1][0] * elem
+            page_stride, run_stride = t.stride(0) * elem, run_stride * elem
+            unit = 16
+            while any(v % unit for v in (t.data_ptr(), page_stride, run_stride, run)):
+                unit //= 2
+            if runs >= 1 << 31 or run // unit >= 1 << 31:
+                raise ValueError("a page is too large")
+            rows.append(_TENSOR.pack(t.data_ptr(), page_stride, run_stride, runs, run // unit,
+                                     unit, chunk0))
+            chunk0 += -(-runs * (run // unit) // CHUNK_UNITS)
+        if chunk0 >= 1 << 30:
+            raise ValueError("the pages are too large")
+        self._chunks = chunk0
+        host = torch.frombuffer(bytearray(b"".join(rows)), dtype=torch.uint8)
+        self._descriptors = host.to(self.device)
+
+    def _bind_meta(self, sizes: List[int], words: int) -> None:
+        parts = self.meta.split(sizes)
+        self._header = parts[0]
+        self.refs, self.lengths = parts[1][:self.pages], parts[2][:self.slots]
+        self.table = parts[3][:self.slots * self.width].view(self.slots, self.width)
+        self._free_bits, self._stale_bits = parts[4][:words], parts[5][:words]
+
+    # -- books from the host ------------------------------------------------------------------
+    def bind(self, table, lengths) -> "PagePool":
+        """Take over sequences whose pages are already in the tensors: ``table`` ``[slots, <=
+        width]`` and ``lengths`` ``[slots]``.  Waits for the device."""
+        table = torch.as_tensor(table).cpu().numpy().astype(np.int64)
+        lengths = torch.as_tensor(lengths).cpu().numpy().astype(np.int64)
+        if table.ndim != 2 or table.shape[0] != self.slots or table.shape[1] > self.width \
+                or lengths.shape != (self.slots,):
+            raise ValueError("table must be [%d, <= %d], lengths [%d]" % (
+                self.slots, self.width, self.slots))
+        if (lengths < 0).any() or (lengths > min(table.shape[1] * self.page_tokens,
+                                                 (1 << 31) - 1)).any():
+            raise ValueError("a length is negative or longer than its row of the table")
+        held = np.arange(table.shape[1]) < -(-lengths // self.page_tokens)[:, None]
+        if ((table < 0) | (table >= self.pages))[held].any():
+            raise ValueError("a page of the table is out of range")
+        books = np.full((self.slots, self.width), -1, np.int32)
+        books[:, :table.shape[1]] = np.where(held, table, -1)
+        self._write_books(books, lengths.astype(np.int32))
+        return self
+
+    def _write_books(self, table: np.ndarray, lengths: np.ndarray) -> None:
+        refs = np.bincount(table[table >= 0].astype(np.int64), minlength=self.pages)
+        free = refs == 0
+        words = self._free_bits.numel()
+        packed = np.packbits(np.pad(free, (0, 32 * words - self.pages)), bitorder="little")
+        header = np.zeros(HEADER, np.int32)
+        header[_FREE] = int(free.sum())
+        for part, value in ((self._header, header), (self.refs, refs.astype(np.int32)),
+                            (self.lengths, lengths), (self.table, table),
+                            (self._free_bits, packed.view(np.int32)),
+                            (self._stale_bits, packed.view(np.int32))):
+            part.copy_(torch.from_numpy(np.ascontiguousarray(value)))
+
+    # -- operations ---------------------------------------------------------------------------
+    def _numbers(self, what: str, values: Numbers, limit: int, distinct: bool = False):
+        """``values`` as a contiguous integer tensor on the pool's device."""
+        if isinstance(values, torch.Tensor):
+            if values.dtype not in (torch.int32, torch.int64) or values.dim() != 1:
+                raise TypeError("%s must be a one-dimensional int32 or int64 tensor" % what)
+            if values.device != self.device:
+                raise ValueError("%s must be on %s" % (what, self.device))
+            out = values.contiguous()
+            if self.device.type == "cuda":
+                return out
+            out = out.to(torch.int64)
+        else:
+            out = torch.tensor([int(v) for v in values], dtype=torch.int64)
+        host = out.tolist()
+        if any(not 0 <= v < limit for v in host):
+            raise ValueError("%s must be in [0, %d)" % (what, limit))
+        if distinct and len(set(host)) != len(host):
+            raise ValueError("%s must be distinct" % what)
+        return out.to(self.device)
+
+    def _enqueue(self, name: str, *args) -> None:
+        if self.device.type == "cuda":
+            lib = hip()
+            with torch.cuda.device(self.device):
+                lib.check(getattr(lib, "tpi_pages_" + name)(
+                    self._args, *args, torch.cuda.current_stream().cuda_stream), name)
+            return
+        getattr(native(), "pages_" + name)(self._args, *args)
+        self.check()
+
+    def _pair(self, name: str, src, dst) -> None:
+        if src.shape != dst.shape:
+            raise ValueError("%s needs as many sources as destinations" % name)
+        if src.dtype != dst.dtype:
+            src, dst = src.to(torch.int64), dst.to(torch.int64)
+        args = (src.data_ptr(), dst.data_ptr(), src.numel())
+        if self.device.type == "cuda":
+            args += (int(src.dtype == torch.int64),)
+        self._enqueue(name, *args)
+
+    def _limit(self, name: str, count: int) -> None:
+        if count > self.slots:  # some slot is named twice
+            raise ValueError("%s of %d slots, the pool has %d" % (name, count, self.slots))
+
+    def copy(self, src: Numbers, dst: Numbers) -> None:
+        """Page ``src[i]`` to page ``dst[i]`` in every tensor; the books stay as they are.  No page
+        may be a destination twice, nor destination and source: of such a call on device numbers,
+        those destinations' content is undefined.  A pair with a number out of range is left
+        out."""
+        known = self.device.type == "cpu" or not (isinstance(src, torch.Tensor) or
+                                                  isinstance(dst, torch.Tensor))
+        if known and set(map(int, src)) & set(map(int, dst)):
+            raise ValueError("a page is both source and destination")
+        src = self._numbers("source pages", src, self.pages)
+        dst = self._numbers("destination pages", dst, self.pages, distinct=True)
+        self._pair("copy", src, dst)
+
+    def fork(self, src: Numbers, dst: Numbers) -> None:
+        """Slot ``dst[i]``, empty so far, becomes a copy of slot ``src[i]``'s sequence: it shares its
+        full pages, and has a copy of a partial last page (either may go on writing).  A source may
+        be named more than once; all are taken as they were before the call."""
+        src = self._numbers("source slots", src, self.slots)
+        dst = self._numbers("destination slots", dst, self.slots, distinct=True)
+        self._limit("fork", dst.numel())
+        self._pair("fork", src, dst)
+
+    def extend(self, slots: Numbers, tokens: Union[int, Numbers]) -> None:
+        """Slot ``slots[i]``'s sequence grows by ``tokens`` (``tokens[i]``) tokens: its row of the
+        table gets the pages for them, lowest free number first.  The new tokens' bytes are
+        whatever the pages held."""
+        slots = self._numbers("slots", slots, self.slots, distinct=True)
+        self._limit("extend", slots.numel())
+        each, more = 0, None
+        if isinstance(tokens, int):
+            each = tokens
+            if not 0 <= each < 1 << 31:
+                raise ValueError("tokens must be in [0, 2^31)")
+        else:
+            more = self._numbers("tokens", tokens, 1 << 31)
+            if more.shape != slots.shape:
+                raise ValueError("extend needs as many token counts as slots")
+        if self.device.type == "cuda":
+            wide = int(slots.dtype == torch.int64)
+            if more is not None:
+                wide |= 2 * int(more.dtype == torch.int64)
+            self._enqueue("extend", slots.data_ptr(), slots.numel(), wide,
+                          None if more is None else more.data_ptr(), each)
+            return
+        if more is None:
+            more = torch.full_like(slots, each)
+        self._enqueue("extend", slots.data_ptr(), more.data_ptr(), slots.numel())
+
+    def free(self, slots: Numbers) -> None:
+        """The slots' sequences end: pages that no other sequence names become free.  A free slot
+        stays free."""
+        slots = self._numbers("slots", slots, self.slots, distinct=True)
+        self._limit("free", slots.numel())
+        args = (slots.data_ptr(), slots.numel())
+        if self.device.type == "cuda":
+            args += (int(slots.dtype == torch.int64),)
+        self._enqueue("free", *args)
+
+    def compact(self, clear: bool = False) -> None:
+        """Move the live pages to numbers 0, 1, ... (as few moves as there are holes among them) and
+        rewrite the table.  ``clear``: also fill free pages with zeros, those that have been
+        written since the last time."""
+        self._enqueue("compact", int(clear) if self.device.type == "cuda" else bool(clear))
+
+    # -- what the host may know ---------------------------------------------------------------
+    def check(self) -> None:
+        """Raise :class:`PageError` if an operation has been refused since the last check.  Waits for
+        the device."""
+        code = int(self._header[_ERROR])
+        if code:
+            self._header[_ERROR] = 0
+            raise PageError(_ERRORS.get(code, "error %d" % code))
+
+    def status(self) -> Dict[str, Any]:
+        """``{"pages", "free", "live", "error"}``; waits for the device."""
+        free, code = self._header[:2].tolist()
+        return {"pages": self.pages, "free": free, "live": self.pages - free,
+                "error": _ERRORS.get(code, "error %d" % code) if code else None}
