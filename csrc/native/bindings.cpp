@@ -11,7 +11,7 @@
 #include "../common/tpz.h"
 #include "fileio.h"
 #include "hostops.h"
-#include "stateops.h"
+#include "pages.h"
 #include "transfer.h"
 
 namespace py = pybind11;
@@ -178,14 +178,8 @@ PYBIND11_MODULE(_tpi_native, m) {
     }
     return py::make_tuple(bad, first);
   });
-  m.attr("DROPOUT_ARGS_SIZE") = (int)sizeof(tpi_dropout_args);
   m.attr("PAGES_SIZE") = (int)sizeof(tpi_pages);
   m.attr("PAGE_TENSOR_SIZE") = (int)sizeof(tpi_page_tensor);
-  m.def("dropout", [](const py::bytes& args, int threads) {
-    const tpi_dropout_args a = struct_of<tpi_dropout_args>(args);
-    py::gil_scoped_release nogil;
-    tpi::dropout(a, threads);
-  });
   m.def("pages_copy", [](const py::bytes& pool, uintptr_t src, uintptr_t dst, int64_t n) {
     tpi::pages_copy(struct_of<tpi_pages>(pool), (const int64_t*)src, (const int64_t*)dst, n);
   });

@@ -1,89 +1,13 @@
-// Host (CPU) implementations of the operators on a rank's state: dropout from a counter-based
-// generator and the pages of a paged cache.  They serve CPU ranks and define the results that
-// csrc/hip/dropout.hip and csrc/hip/pages.hip give bit for bit (tests compare both).
-#include "stateops.h"
+// Host (CPU) implementation of the pages of a paged cache.  It serves CPU ranks and defines the
+// results that csrc/hip/pages.hip gives bit for bit (tests compare both).
+#include "pages.h"
 
 #include <string.h>
 
 #include <algorithm>
-#include <thread>
 #include <vector>
 
-#include "../common/float16.h"
-#include "../common/philox.h"
-
 namespace tpi {
-
-namespace {
-
-inline float load(const void* base, int64_t at, int type) {
-  if (type == TPI_F32) return ((const float*)base)[at];
-  const uint16_t h = ((const uint16_t*)base)[at];
-  return type == TPI_F16 ? tpi_f16_to_f32(h) : tpi_bf16_to_f32(h);
-}
-
-inline void store(void* base, int64_t at, int type, float v) {
-  if (type == TPI_F32) ((float*)base)[at] = v;
-  else ((uint16_t*)base)[at] = type == TPI_F16 ? tpi_f32_to_f16(v) : tpi_f32_to_bf16(v);
-}
-
-void dropout_range(const tpi_dropout_args& a, uint64_t seed, uint64_t draw, uint64_t lo,
-                   uint64_t hi) {
-  int64_t index[TPI_MAX_DIMS];
-  uint64_t rest = lo;
-  for (int d = a.ndim - 1; d >= 0; --d) {
-    index[d] = (int64_t)(rest % (uint64_t)a.sizes[d]);
-    rest /= (uint64_t)a.sizes[d];
-  }
-  uint64_t block = ~0ull;
-  uint32_t kept = 0;
-  for (uint64_t e = lo; e < hi; ++e) {
-    int64_t x = 0, r = 0, o = 0;
-    uint64_t n = a.first;
-    for (int d = 0; d < a.ndim; ++d) {
-      x += index[d] * a.sx[d];
-      r += index[d] * a.sr[d];
-      o += index[d] * a.so[d];
-      n += (uint64_t)(index[d] * a.si[d]);
-    }
-    if (n >> 3 != block) {
-      block = n >> 3;
-      kept = tpi_draw_block(block, draw, seed, a.threshold);
-    }
-    float v = 0.0f;
-    if (kept >> (n & 7) & 1) v = load((const void*)a.x, x, a.in_type) * a.scale;
-    if (a.residual) v = v + load((const void*)a.residual, r, a.out_type);
-    store((void*)a.out, o, a.out_type, v);
-    for (int d = a.ndim - 1; d >= 0 && ++index[d] == a.sizes[d]; --d) index[d] = 0;
-  }
-}
-
-}  // namespace
-
-void dropout(const tpi_dropout_args& a, int threads) {
-  uint64_t seed = a.seed, draw = a.draw, total = 1;
-  if (a.state) {
-    seed = ((const uint64_t*)a.state)[0];
-    draw = ((const uint64_t*)a.state)[1] + a.draw;
-  }
-  if (a.used) {
-    ((uint64_t*)a.used)[0] = seed;
-    ((uint64_t*)a.used)[1] = draw;
-  }
-  for (int d = 0; d < a.ndim; ++d) total *= (uint64_t)a.sizes[d];
-  const uint64_t least = 1 << 16;  // elements worth a thread
-  const int count = (int)std::max<uint64_t>(
-      1, std::min<uint64_t>((uint64_t)std::max(1, threads), total / least));
-  std::vector<std::thread> pool;
-  for (int t = 1; t < count; ++t)
-    pool.emplace_back([&, t] {
-      dropout_range(a, seed, draw, total * t / count, total * (t + 1) / count);
-    });
-  dropout_range(a, seed, draw, 0, total / count);
-  for (auto& t : pool) t.join();
-}
-
-// ---- pages ---------------------------------------------------------------------------------------
 
 namespace {
 

@@ -5,10 +5,8 @@
 
 namespace tpi {
 
-// Host implementations of csrc/hip/dropout.hip and csrc/hip/pages.hip, bit for bit; addresses
-// in the arguments are host memory.  The pages' functions give the reason of a refusal in the
-// pool's header, as the kernels do.
-void dropout(const tpi_dropout_args& a, int threads);
+// Host implementations of csrc/hip/pages.hip; addresses in `p` are host memory.  The reason of a
+// refusal goes to the pool's header, as the kernels do it.
 void pages_copy(const tpi_pages& p, const int64_t* src, const int64_t* dst, int64_t n);
 void pages_fork(const tpi_pages& p, const int64_t* src, const int64_t* dst, int64_t n);
 void pages_extend(const tpi_pages& p, const int64_t* slots, const int64_t* more, int64_t n);

@@ -10,6 +10,8 @@
 
 #include <vector>
 
+#include "torchext.h"
+
 namespace {
 
 at::Tensor empty_nogil(const std::vector<int64_t>& shape, const at::Tensor& like) {
@@ -20,8 +22,42 @@ at::Tensor empty_nogil(const std::vector<int64_t>& shape, const at::Tensor& like
 
 }  // namespace
 
+namespace tpi {
+
+static HipApi g_hip;
+
+const HipApi& hip_api() {
+  if (!g_hip.dropout) throw HipFailure("libtpi_hip.so is not loaded");
+  return g_hip;
+}
+
+void hip_check(int rc, const char* what) {
+  if (rc != 0) throw HipFailure(std::string(what) + " failed: " + hip_api().last_error());
+}
+
+}  // namespace tpi
+
 PYBIND11_MODULE(_tpi_torch, m) {
-  m.doc() = "torch helpers that release the GIL (terraform_provider_iterative_amd)";
+  m.doc() = "torch helpers that release the GIL, torch operators and their launches "
+            "(terraform_provider_iterative_amd)";
+  py::register_local_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const tpi::HipFailure& e) {
+      const auto type =
+          py::module_::import("terraform_provider_iterative_amd.ops._loader").attr("HipError");
+      PyErr_SetString(type.ptr(), e.what());
+    }
+  });
+  m.def("use_hip", [](const std::vector<uintptr_t>& at) {
+    if (at.size() != 7) throw std::invalid_argument("use_hip: addresses of 7 entry points");
+    tpi::g_hip = {(decltype(&tpi_last_error))at[0],  (decltype(&tpi_dropout))at[1],
+                  (decltype(&tpi_pages_copy))at[2],  (decltype(&tpi_pages_fork))at[3],
+                  (decltype(&tpi_pages_extend))at[4], (decltype(&tpi_pages_free))at[5],
+                  (decltype(&tpi_pages_compact))at[6]};
+  });
+  tpi::bind_dropout(m);
+  tpi::bind_pages(m);
   m.def("empty", &empty_nogil, "at::empty(shape, like.options()) with the GIL released",
         py::arg("shape"), py::arg("like"));
 }

@@ -256,8 +256,8 @@ def build_stager(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
-    """``_tpi_torch``: torch helpers that release the GIL (``csrc/torchext``; host code against
-    torch's own headers and libraries, same C++ ABI)."""
+    """``_tpi_torch``: torch helpers that release the GIL, torch operators and their launches
+    (``csrc/torchext``; host code against torch's own headers and libraries, same C++ ABI)."""
     srcs = _sources("torchext/*.cpp")
     if not srcs:
         return ""
@@ -268,15 +268,30 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     tl = torch_lib_dir()
     cxx = os.environ.get("CXX", "g++")
-    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           "-DTORCH_EXTENSION_NAME=_tpi_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-isystem", sysconfig.get_paths()["include"], *srcs, "-L" + tl, "-Wl,-rpath," + tl,
-           "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", "@OUT@"]
+    flags = [cxx, "-O3", "-std=c++17", "-fPIC", "-Wall", "-pthread",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",  # c10's stream of a device
+             "-isystem", os.path.join(os.path.dirname(ROCM_LIB), "include"),
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+             "-DTORCH_EXTENSION_NAME=_tpi_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+             "-isystem", sysconfig.get_paths()["include"]]
     # torch's version file is a dependency: a different torch needs a rebuild
-    deps = srcs + [os.path.join(os.path.dirname(torch.__file__), "version.py")]
-    return _build(TORCH_EXT, cmd, deps, force, verbose)
+    headers = _sources("torchext/*.h", "common/*.h", "hip/tpi_hip.h") + [
+        os.path.join(os.path.dirname(torch.__file__), "version.py")]
+    objdir = os.path.join(LIB, "obj")
+    os.makedirs(objdir, exist_ok=True)
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(objdir, "torchext_%s.o" % os.path.basename(src))
+        return _build(obj, [*flags, "-c", src, "-o", "@OUT@"], [src] + headers, force, verbose)
+
+    from concurrent.futures import ThreadPoolExecutor
+
+    with ThreadPoolExecutor(len(srcs)) as pool:  # torch's headers take a minute per source
+        objs = list(pool.map(compile_one, srcs))
+    cmd = [cxx, "-shared", "-fPIC", "-pthread", *objs, "-L" + tl, "-Wl,-rpath," + tl, "-lc10",
+           "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", "@OUT@"]
+    return _build(TORCH_EXT, cmd, objs, force, verbose)
 
 
 def build_all(force: bool = False, verbose: bool = False, hip: bool = True) -> List[str]:

@@ -49,7 +49,7 @@ _torch_ext = None
 
 def torch_ext():
     """``_tpi_torch`` (``csrc/torchext``): torch helpers that release the GIL, e.g.
-    ``empty(shape, like)``.  Loaded after ``import torch`` (it links torch's libraries)."""
+    ``empty(shape, like)``, and torch operators.  Loaded after ``import torch`` (it links torch's libraries)."""
     global _torch_ext
     if _torch_ext is not None:
         return _torch_ext
@@ -67,6 +67,23 @@ def torch_ext():
             spec.loader.exec_module(module)
             _torch_ext = module
     return _torch_ext
+
+
+_torch_hip = None
+
+
+def torch_hip():
+    """:func:`torch_ext` with libtpi_hip.so handed to it: what device tensors need."""
+    global _torch_hip
+    if _torch_hip is None:
+        import ctypes
+
+        lib, ext = hip(), torch_ext()
+        ext.use_hip([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "tpi_last_error", "tpi_dropout", "tpi_pages_copy", "tpi_pages_fork",
+            "tpi_pages_extend", "tpi_pages_free", "tpi_pages_compact")])
+        _torch_hip = ext
+    return _torch_hip
 
 
 class HipError(RuntimeError):

@@ -11,22 +11,18 @@ element's index in the whole tensor (the definition is in ``csrc/common/philox.h
   with another number of ranks goes on with the same masks.
 
 Device tensors go through ``csrc/hip/dropout.hip``, host tensors through
-``csrc/native/stateops.cpp``; both give the same bits.
+``csrc/torchext/dropout.cpp``, which is also the autograd node; both give the same bits.
 """
 from __future__ import annotations
 
-import struct
 from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ._loader import hip, native
-from .packing import MAX_DIMS
+from ._loader import torch_ext, torch_hip
 
-_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # TPI_F32 .. TPI_BF16
-_ARGS = struct.Struct("<9Q%dqf3i" % (5 * MAX_DIMS))  # tpi_dropout_args
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 _WHOLE = 1 << 32
-_PAD = (0,) * MAX_DIMS
 
 
 class Draw(NamedTuple):
@@ -135,31 +131,8 @@ def keep_threshold(p: float) -> Tuple[int, float]:
     return threshold, (_WHOLE / threshold if threshold else 0.0)
 
 
-def _merged(shape: Sequence[int], *strides: Sequence[int]) -> List[Tuple[int, ...]]:
-    """``(size, stride of each operand)`` dims, size-1 dims dropped and dims merged that every
-    operand walks as one."""
-    dims: List[Tuple[int, ...]] = []
-    for dim in zip(shape, *strides):
-        size = dim[0]
-        if size == 1:
-            continue
-        if dims and all(a == b * size for a, b in zip(dims[-1][1:], dim[1:])):
-            dims[-1] = (dims[-1][0] * size,) + dim[1:]
-        else:
-            dims.append(dim)
-    return dims or [(1,) * (1 + len(strides))]
-
-
-class _Plan(NamedTuple):
-    threshold: int
-    scale: float
-    first: int                            # index of the view's first element in the whole tensor
-    strides: Optional[Tuple[int, ...]]    # index strides, None: the view is the whole tensor
-
-
-def _shard_plan(shape, shard) -> Tuple[int, Optional[Tuple[int, ...]]]:
-    if shard is None:
-        return 0, None
+def _shard_walk(shape, shard) -> Tuple[int, List[int]]:
+    """Index of a shard's first element in the whole tensor, and its index strides."""
     whole, starts = (tuple(int(v) for v in part) for part in shard)
     if len(whole) != len(shape) or len(starts) != len(shape):
         raise ValueError("shard must give a size and a start for each of the %d dimensions"
@@ -173,79 +146,7 @@ def _shard_plan(shape, shard) -> Tuple[int, Optional[Tuple[int, ...]]]:
         step *= size
     if step >= 1 << 63:
         raise ValueError("the whole tensor is too large")
-    return first, tuple(reversed(strides))
-
-
-def _contiguous_strides(shape) -> Tuple[int, ...]:
-    out, step = [], 1
-    for size in reversed(shape):
-        out.append(step)
-        step *= size
-    return tuple(reversed(out))
-
-
-def _apply(x, residual, out_dtype, plan: _Plan, draw: Draw, used=None):
-    """One pass: ``(kept ? x * scale : 0) + residual`` in ``out_dtype``."""
-    out = torch.empty_like(x if residual is None else residual, dtype=out_dtype)
-    if x.numel() == 0:  # nor will the backward pass read `used`
-        return out
-    if plan.strides is None and x.is_contiguous() and out.is_contiguous() and (
-            residual is None or residual.is_contiguous()):
-        n = x.numel()
-        ndim, sizes, ones = 1, (n,) + _PAD[1:], (1,) + _PAD[1:]
-        walk = sizes + ones * 4
-    else:
-        index = plan.strides if plan.strides is not None else _contiguous_strides(x.shape)
-        operands = [x.stride(), out.stride() if residual is None else residual.stride(),
-                    out.stride(), index]
-        dims = _merged(x.shape, *operands)
-        ndim = len(dims)
-        if ndim > MAX_DIMS:
-            raise ValueError("tensors with more than %d (merged) dims are not supported" % MAX_DIMS)
-        walk = ()
-        for column in zip(*dims):
-            walk += tuple(column) + _PAD[ndim:]
-    state, seed = draw.state, draw.seed
-    args = _ARGS.pack(x.data_ptr(), 0 if residual is None else residual.data_ptr(),
-                      out.data_ptr(), 0 if state is None else state.data_ptr(),
-                      0 if used is None else used.data_ptr(), seed, draw.number, plan.first,
-                      plan.threshold, *walk, plan.scale, _TYPES[x.dtype], _TYPES[out_dtype], ndim)
-    if x.device.type == "cuda":
-        lib = hip()
-        with torch.cuda.device(x.device):
-            lib.check(lib.tpi_dropout(args, torch.cuda.current_stream().cuda_stream), "dropout")
-    else:
-        native().dropout(args, torch.get_num_threads())
-    return out
-
-
-class _Dropout(torch.autograd.Function):
-    """The gradient of a dropped element is 0, of a kept one the scale times the output's: the
-    operator itself, applied to the gradient (so it can be differentiated again)."""
-
-    @staticmethod
-    def forward(ctx, x, residual, out_dtype, plan, draw):
-        ctx.plan, ctx.draw, ctx.x_dtype = plan, draw, x.dtype
-        used = None
-        if draw.state is not None and ctx.needs_input_grad[0]:
-            # the state may have moved on by the time the backward pass runs
-            used = torch.empty(2, dtype=torch.int64, device=x.device)
-            ctx.draw = Draw(0, 0, used)
-        return _apply(x, residual, out_dtype, plan, draw, used)
-
-    @staticmethod
-    def backward(ctx, grad):
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _run(grad, None, ctx.x_dtype, ctx.plan, ctx.draw)
-        return dx, grad if ctx.needs_input_grad[1] else None, None, None, None
-
-
-def _run(x, residual, out_dtype, plan, draw):
-    if torch.is_grad_enabled() and (x.requires_grad or
-                                    (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, out_dtype, plan, draw)
-    return _apply(x, residual, out_dtype, plan, draw)
+    return first, strides[::-1]
 
 
 def dropout(x: torch.Tensor, p: float, draw: Union[MaskStream, Draw, Tuple[int, int]], *,
@@ -266,12 +167,11 @@ def dropout(x: torch.Tensor, p: float, draw: Union[MaskStream, Draw, Tuple[int, 
 
     The result is enqueued on the current stream of ``x``'s device.
     """
-    if not isinstance(x, torch.Tensor) or x.device.type not in ("cuda", "cpu"):
+    if not isinstance(x, torch.Tensor) or not (x.is_cuda or x.is_cpu):
         raise TypeError("dropout needs a tensor on the GPU or the host")
     if x.dtype not in _TYPES:
         raise TypeError("dropout of %s is not supported (float32, float16, bfloat16)" % x.dtype)
     threshold, scale = keep_threshold(p)
-    out_dtype = x.dtype
     if residual is not None:
         if not isinstance(residual, torch.Tensor) or residual.device != x.device:
             raise ValueError("the residual must be a tensor on %s" % x.device)
@@ -280,13 +180,13 @@ def dropout(x: torch.Tensor, p: float, draw: Union[MaskStream, Draw, Tuple[int, 
                              % (tuple(residual.shape), tuple(x.shape)))
         if residual.dtype not in (x.dtype, torch.float32):
             raise TypeError("the residual must be %s or float32" % x.dtype)
-        out_dtype = residual.dtype
-    first, strides = _shard_plan(x.shape, shard)
+    first, strides = (0, ()) if shard is None else _shard_walk(x.shape, shard)
     draw = _as_draw(draw)
     if draw.state is not None and draw.state.device != x.device:
         raise ValueError("the mask stream is on %s, the tensor on %s" % (draw.state.device,
                                                                          x.device))
-    return _run(x, residual, out_dtype, _Plan(threshold, scale, first, strides), draw)
+    ext = torch_hip() if x.is_cuda else torch_ext()
+    return ext.dropout(x, residual, threshold, scale, *draw, first, strides)
 
 
 class CounterDropout(torch.nn.Module):

@@ -8,7 +8,7 @@ host, so they can be captured into a graph; the host reads the books when it ask
 (:meth:`PagePool.status`).
 
 Results are the same on every run and on the host (``csrc/hip/pages.hip``,
-``csrc/native/stateops.cpp``): free pages are taken lowest number first, in the order in which
+``csrc/native/pages.cpp``): free pages are taken lowest number first, in the order in which
 sequences are named.
 
 The books are one int32 tensor (:attr:`PagePool.meta`).  ``TrainingState(paged={"kv": pool})``
@@ -23,7 +23,7 @@ from typing import Any, Dict, List, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from ._loader import hip, native
+from ._loader import native, torch_hip
 from .packing import canonical_view
 
 HEADER, CHUNK_UNITS = 16, 1024  # TPI_PAGES_HEADER, TPI_PAGE_UNITS
@@ -77,6 +77,7 @@ class PagePool:
         self.device = tensors[0].device
         if self.device.type not in ("cuda", "cpu"):
             raise ValueError("a pool's tensors must be on the GPU or the host")
+        self._on_device = self.device.type == "cuda"
         if any(t.dim() < 2 or t.numel() == 0 for t in tensors):
             raise ValueError("a pool's tensors need a page dimension and bytes in each page")
         if len({(t.device, t.shape[0]) for t in tensors}) != 1:
@@ -188,7 +189,7 @@ class PagePool:
             if values.device != self.device:
                 raise ValueError("%s must be on %s" % (what, self.device))
             out = values.contiguous()
-            if self.device.type == "cuda":
+            if self._on_device:
                 return out
             out = out.to(torch.int64)
         else:
@@ -201,11 +202,8 @@ class PagePool:
         return out.to(self.device)
 
     def _enqueue(self, name: str, *args) -> None:
-        if self.device.type == "cuda":
-            lib = hip()
-            with torch.cuda.device(self.device):
-                lib.check(getattr(lib, "tpi_pages_" + name)(
-                    self._args, *args, torch.cuda.current_stream().cuda_stream), name)
+        if self._on_device:
+            getattr(torch_hip(), "pages_" + name)(self._args, self.device.index, *args)
             return
         getattr(native(), "pages_" + name)(self._args, *args)
         self.check()
@@ -216,7 +214,7 @@ class PagePool:
         if src.dtype != dst.dtype:
             src, dst = src.to(torch.int64), dst.to(torch.int64)
         args = (src.data_ptr(), dst.data_ptr(), src.numel())
-        if self.device.type == "cuda":
+        if self._on_device:
             args += (int(src.dtype == torch.int64),)
         self._enqueue(name, *args)
 
@@ -229,7 +227,7 @@ class PagePool:
         may be a destination twice, nor destination and source: of such a call on device numbers,
         those destinations' content is undefined.  A pair with a number out of range is left
         out."""
-        known = self.device.type == "cpu" or not (isinstance(src, torch.Tensor) or
+        known = not self._on_device or not (isinstance(src, torch.Tensor) or
                                                   isinstance(dst, torch.Tensor))
         if known and set(map(int, src)) & set(map(int, dst)):
             raise ValueError("a page is both source and destination")
@@ -261,12 +259,12 @@ class PagePool:
             more = self._numbers("tokens", tokens, 1 << 31)
             if more.shape != slots.shape:
                 raise ValueError("extend needs as many token counts as slots")
-        if self.device.type == "cuda":
+        if self._on_device:
             wide = int(slots.dtype == torch.int64)
             if more is not None:
                 wide |= 2 * int(more.dtype == torch.int64)
             self._enqueue("extend", slots.data_ptr(), slots.numel(), wide,
-                          None if more is None else more.data_ptr(), each)
+                          0 if more is None else more.data_ptr(), each)
             return
         if more is None:
             more = torch.full_like(slots, each)
@@ -278,7 +276,7 @@ class PagePool:
         slots = self._numbers("slots", slots, self.slots, distinct=True)
         self._limit("free", slots.numel())
         args = (slots.data_ptr(), slots.numel())
-        if self.device.type == "cuda":
+        if self._on_device:
             args += (int(slots.dtype == torch.int64),)
         self._enqueue("free", *args)
 
@@ -286,7 +284,7 @@ class PagePool:
         """Move the live pages to numbers 0, 1, ... (as few moves as there are holes among them) and
         rewrite the table.  ``clear``: also fill free pages with zeros, those that have been
         written since the last time."""
-        self._enqueue("compact", int(clear) if self.device.type == "cuda" else bool(clear))
+        self._enqueue("compact", int(clear) if self._on_device else bool(clear))
 
     # -- what the host may know ---------------------------------------------------------------
     def check(self) -> None:

@@ -34,7 +34,6 @@ def test_philox_known_answers():
 
 
 def test_argument_blocks_match_the_c_structs():
-    assert masking._ARGS.size == ops.native().DROPOUT_ARGS_SIZE
     assert paging._POOL.size == ops.native().PAGES_SIZE
     assert paging._TENSOR.size == ops.native().PAGE_TENSOR_SIZE
 
