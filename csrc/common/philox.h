@@ -30,6 +30,14 @@ struct tpi_philox_words {
   uint32_t w[4];
 };
 
+TPI_PHD static inline uint32_t tpi_xor3(uint32_t a, uint32_t b, uint32_t c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction
+#else
+  return a ^ b ^ c;
+#endif
+}
+
 TPI_PHD static inline tpi_philox_words tpi_philox(uint64_t block, uint64_t draw, uint32_t level,
                                                   uint64_t seed) {
   uint32_t a = (uint32_t)block, b = (uint32_t)(block >> 32);
@@ -38,9 +46,9 @@ TPI_PHD static inline tpi_philox_words tpi_philox(uint64_t block, uint64_t draw,
 #pragma GCC unroll 10
   for (int r = 0; r < TPI_PHILOX_ROUNDS; ++r) {
     const uint64_t p = (uint64_t)TPI_PHILOX_M0 * a, q = (uint64_t)TPI_PHILOX_M1 * c;
-    a = (uint32_t)(q >> 32) ^ b ^ k0;
+    a = tpi_xor3((uint32_t)(q >> 32), b, k0);
     b = (uint32_t)q;
-    c = (uint32_t)(p >> 32) ^ d ^ k1;
+    c = tpi_xor3((uint32_t)(p >> 32), d, k1);
     d = (uint32_t)p;
     k0 += TPI_PHILOX_W0;
     k1 += TPI_PHILOX_W1;
@@ -53,22 +61,36 @@ TPI_PHD static inline uint32_t tpi_philox_half(const tpi_philox_words& p, int la
   return (p.w[lane >> 1] >> (16 * (lane & 1))) & 0xffffu;
 }
 
-// Bit j: element j of the block is kept.  `threshold` is 0 .. 2^32 (the share kept * 2^32).
-TPI_PHD static inline uint32_t tpi_draw_block(uint64_t block, uint64_t draw, uint64_t seed,
-                                              uint64_t threshold) {
-  const tpi_philox_words p = tpi_philox(block, draw, 0, seed);
-  const uint32_t hi = (uint32_t)(threshold >> 16), lo = (uint32_t)threshold & 0xffffu;
+// A threshold of 0 .. 2^32 (the share kept * 2^32) as two halves that a half-word is compared
+// with: kept below `high`, and at `high` if level 1's half-word is below `low`.  All kept (2^32)
+// is "at 0xffff, any": `high` stays a half-word.
+struct tpi_keep {
+  uint32_t high, low;
+};
+
+TPI_PHD static inline tpi_keep tpi_keep_below(uint64_t threshold) {
+  if (threshold >> 32) return tpi_keep{0xffffu, 0x10000u};
+  return tpi_keep{(uint32_t)(threshold >> 16), (uint32_t)threshold & 0xffffu};
+}
+
+// Bit j: element j of the block is kept.  `p` is level 0 of the block.
+TPI_PHD static inline uint32_t tpi_kept_bits(const tpi_philox_words& p, uint64_t block,
+                                             uint64_t draw, uint64_t seed, tpi_keep keep) {
   uint32_t kept = 0, tie = 0;
-#pragma GCC unroll 8
   for (int j = 0; j < TPI_DRAW_LANES; ++j) {
     const uint32_t h = tpi_philox_half(p, j);
-    kept |= (uint32_t)(h < hi) << j;
-    tie |= (uint32_t)(h == hi) << j;
+    kept |= (uint32_t)(h < keep.high) << j;
+    tie |= (uint32_t)(h == keep.high) << j;
   }
-  if (tie && lo) {
+  if (tie) {
     const tpi_philox_words q = tpi_philox(block, draw, 1, seed);
     for (int j = 0; j < TPI_DRAW_LANES; ++j)
-      kept |= (tie >> j & 1u & (uint32_t)(tpi_philox_half(q, j) < lo)) << j;
+      kept |= (tie >> j & 1u & (uint32_t)(tpi_philox_half(q, j) < keep.low)) << j;
   }
   return kept;
+}
+
+TPI_PHD static inline uint32_t tpi_draw_block(uint64_t block, uint64_t draw, uint64_t seed,
+                                              tpi_keep keep) {
+  return tpi_kept_bits(tpi_philox(block, draw, 0, seed), block, draw, seed, keep);
 }

@@ -8,7 +8,7 @@
 // one rounding to the output's type.  A dropped element is 0 whatever x holds (NaN, infinity).
 //
 //  k_dropout_rows     rows of unit stride (a contiguous tensor is one row).  A thread owns the 8
-//                     elements of one generator block.
+//                     elements of a generator block: one 16-byte access (two for fp32) each way.
 //  k_dropout_strided  anything else, one thread per element: its own block of the generator.
 #include <hip/hip_runtime.h>
 
@@ -27,15 +27,23 @@ template <> struct Elem<TPI_F32> { typedef float type; };
 template <> struct Elem<TPI_F16> { typedef _Float16 type; };
 template <> struct Elem<TPI_BF16> { typedef __bf16 type; };
 
+// Division of a number below 2^31 by a constant: (n + high word of n * mul) >> shift, with
+// mul = floor(2^32 (2^shift - d) / d) + 1 and shift the least with 2^shift >= d.
+struct Divider {
+  uint32_t mul, shift;
+};
+
 struct RowArgs {
   const void* x;
   const void* residual;
   void* out;
   const uint64_t* state;
   uint64_t* used;
-  uint64_t seed, draw, threshold, first;
+  uint64_t seed, draw, first;
   int64_t rows, cols, sx, sr, so, si;  // elements
-  uint64_t per_row;                    // generator blocks (threads) per row
+  uint64_t per_row;                    // generator blocks per row
+  Divider by_row;                      // by per_row
+  tpi_keep keep;
   float scale;
 };
 
@@ -69,43 +77,89 @@ __device__ static inline typename Elem<OUT>::type apply(float x, float residual,
   return (typename Elem<OUT>::type)v;
 }
 
-// VEC: every row starts on a block of the generator and on 16 bytes in memory, so a thread's 8
-// elements move as vectors; otherwise element by element, the block's ends cut at the row's.
-template <int IN, int OUT, bool RES, bool VEC>
+// Whether a half-word of the block equals keep.high.
+__device__ static inline bool ties(const tpi_philox_words& p, tpi_keep keep) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t both = keep.high | keep.high << 16;
+  u16x2 least = {1, 1};  // 0 where some half-word is equal
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const u16x2 off = __builtin_bit_cast(u16x2, p.w[k] ^ both);
+    least = __builtin_elementwise_min(least, off);
+  }
+  return __builtin_bit_cast(uint32_t, least) != 0x00010001u;
+}
+
+// 8 elements that may begin at any element: the GPU's vector accesses need no alignment.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+  T e[8];
+};
+
+template <typename T>
+__device__ static inline Eight<T> load8(const T* p) {
+  return *(const Eight<T>*)p;
+}
+
+// Elements of 2 bytes are one 16-byte access, stored nontemporally: the caches keep what is read
+// (16M bf16 elements with a residual 18.5 us instead of 19.6, 8M 10.4 instead of 11.1; loading them
+// so too costs what the last kernel left there: 14.4 us instead of 13.5 without a residual).  Those of
+// 4 bytes are two, each half of what a line's lanes write: nontemporal they cost 99 us, not 92.
+template <typename T>
+__device__ static inline void store8(T* p, Eight<T> v) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint32_t raw __attribute__((ext_vector_type(4), aligned(2)));
+    __builtin_nontemporal_store(__builtin_bit_cast(raw, v), (raw*)p);
+  } else {
+    *(Eight<T>*)p = v;
+  }
+}
+
+// A thread takes one block of the generator (two or four, with all loads in flight first, are 6
+// to 20 % slower: fewer waves than accesses to hide).  Its 20 products are a quarter of what the
+// memory leaves time for: with one round instead of 10 the kernel is 4 % faster.
+template <int IN, int OUT, bool RES>
 __global__ __launch_bounds__(kThreads) void k_dropout_rows(RowArgs a) {
   typedef typename Elem<IN>::type TI;
   typedef typename Elem<OUT>::type TO;
-  typedef TI vin __attribute__((ext_vector_type(8)));
-  typedef TO vout __attribute__((ext_vector_type(8)));
   const Key key = read_key(a.state, a.used, a.seed, a.draw);
   const uint64_t t = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t row = a.rows == 1 ? 0 : (int64_t)(t / a.per_row);
+  int64_t row = 0;
+  if (a.rows > 1)
+    row = t >> 31 ? (int64_t)(t / a.per_row)
+                  : (int64_t)((__umulhi((uint32_t)t, a.by_row.mul) + (uint32_t)t) >>
+                              a.by_row.shift);
   if (row >= a.rows) return;
   const uint64_t b = t - (uint64_t)row * a.per_row;
-  if (b >= a.per_row) return;
-  const TI* x = (const TI*)a.x + row * a.sx;
-  const TO* r = RES ? (const TO*)a.residual + row * a.sr : nullptr;
-  TO* o = (TO*)a.out + row * a.so;
-  const uint64_t start = a.first + (uint64_t)row * (uint64_t)a.si;
-  const int64_t c0 = (int64_t)(b * 8) - (int64_t)(start & 7);  // column of the block's lane 0
+  const uint64_t start = a.first + (uint64_t)row * (uint64_t)a.si, block = (start >> 3) + b;
+  const int64_t c0 = (int64_t)(b * 8) - (int64_t)(start & 7);  // column of the block's element 0
   if (c0 >= a.cols) return;
-  const uint32_t kept = tpi_draw_block((start >> 3) + b, key.draw, key.seed, a.threshold);
-  if (VEC && c0 + 8 <= a.cols) {
-    const vin v = *(const vin*)(x + c0);
-    vout w;
-    if (RES) w = *(const vout*)(r + c0);
+  const TI* x = (const TI*)a.x + row * a.sx + c0;
+  const TO* r = RES ? (const TO*)a.residual + row * a.sr + c0 : nullptr;
+  TO* o = (TO*)a.out + row * a.so + c0;
+  const bool whole = c0 >= 0 && c0 + 8 <= a.cols;
+  Eight<TI> in;
+  Eight<TO> add;
+  if (whole) {
+    in = load8(x);
+    if (RES) add = load8(r);
+  }
+  const tpi_philox_words p = tpi_philox(block, key.draw, 0, key.seed);
+  if (whole && !ties(p, a.keep)) {
+    Eight<TO> out;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      w[j] = apply<OUT, RES>((float)v[j], RES ? (float)w[j] : 0.0f, kept >> j & 1, a.scale);
-    *(vout*)(o + c0) = w;
+      out.e[j] = apply<OUT, RES>((float)in.e[j], RES ? (float)add.e[j] : 0.0f,
+                                 tpi_philox_half(p, j) < a.keep.high, a.scale);
+    store8(o, out);
     return;
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int64_t c = c0 + j;
-    if (c >= 0 && c < a.cols)
-      o[c] = apply<OUT, RES>((float)x[c], RES ? (float)r[c] : 0.0f, kept >> j & 1, a.scale);
-  }
+  // a row's ends, and blocks that need their second number (one in 8192): element by element
+  const uint32_t kept = tpi_kept_bits(p, block, key.draw, key.seed, a.keep);
+#pragma unroll 1
+  for (int j = 0; j < 8; ++j)
+    if (c0 + j >= 0 && c0 + j < a.cols)
+      o[j] = apply<OUT, RES>((float)x[j], RES ? (float)r[j] : 0.0f, kept >> j & 1, a.scale);
 }
 
 template <int IN, int OUT, bool RES>
@@ -113,6 +167,7 @@ __global__ __launch_bounds__(kThreads) void k_dropout_strided(tpi_dropout_args a
   typedef typename Elem<IN>::type TI;
   typedef typename Elem<OUT>::type TO;
   const Key key = read_key((const uint64_t*)a.state, (uint64_t*)a.used, a.seed, a.draw);
+  const tpi_keep keep = tpi_keep_below(a.threshold);
   for (uint64_t e = (uint64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
        e += (uint64_t)gridDim.x * kThreads) {
     uint64_t rest = e, n = a.first;
@@ -126,14 +181,12 @@ __global__ __launch_bounds__(kThreads) void k_dropout_strided(tpi_dropout_args a
       n += (uint64_t)(i * a.si[d]);
       rest = q;
     }
-    const uint32_t kept = tpi_draw_block(n >> 3, key.draw, key.seed, a.threshold);
+    const uint32_t kept = tpi_draw_block(n >> 3, key.draw, key.seed, keep);
     ((TO*)a.out)[o] = apply<OUT, RES>((float)((const TI*)a.x)[x],
                                       RES ? (float)((const TO*)a.residual)[r] : 0.0f,
                                       kept >> (n & 7) & 1, a.scale);
   }
 }
-
-int64_t elem_bytes(int type) { return type == TPI_F32 ? 4 : 2; }
 
 template <int IN, int OUT, bool RES>
 int launch(const tpi_dropout_args& a, hipStream_t stream) {
@@ -158,7 +211,7 @@ int launch(const tpi_dropout_args& a, hipStream_t stream) {
   k.used = (uint64_t*)a.used;
   k.seed = a.seed;
   k.draw = a.draw;
-  k.threshold = a.threshold;
+  k.keep = tpi_keep_below(a.threshold);
   k.first = a.first;
   k.scale = a.scale;
   k.cols = a.sizes[last];
@@ -169,28 +222,28 @@ int launch(const tpi_dropout_args& a, hipStream_t stream) {
     k.so = a.so[0];
     k.si = a.si[0];
   }
-  const auto on16 = [](uint64_t ptr, int64_t stride, int64_t bytes) {
-    return ptr % 16 == 0 && stride * bytes % 16 == 0;
-  };
-  const bool vec = a.first % 8 == 0 && k.si % 8 == 0 && on16(a.x, k.sx, elem_bytes(IN)) &&
-                   on16(a.out, k.so, elem_bytes(OUT)) &&
-                   (!RES || on16(a.residual, k.sr, elem_bytes(OUT)));
-  // a row that starts inside a block touches up to one more of them
-  k.per_row = vec ? (uint64_t)(k.cols + 7) / 8 : (uint64_t)(k.cols + 14) / 8;
-  const uint64_t threads = k.per_row * (uint64_t)k.rows;
-  const uint64_t grid = (threads + kThreads - 1) / kThreads;
+  // blocks that a row touches: its first one begins up to 7 elements before it
+  const uint64_t lead = k.si % 8 == 0 ? a.first % 8 : 7;
+  k.per_row = ((uint64_t)k.cols + lead + 7) / 8;
+  if (k.per_row >> 31 == 0) {
+    while (k.by_row.shift < 31 && (1ull << k.by_row.shift) < k.per_row) ++k.by_row.shift;
+    k.by_row.mul =
+        (uint32_t)(((((1ull << k.by_row.shift) - k.per_row) << 32) / k.per_row) + 1);
+  }
+  const uint64_t blocks = k.per_row * (uint64_t)k.rows;
+  const uint64_t grid = (blocks + kThreads - 1) / kThreads;
   if (grid > 0x7fffffffull) return tpi_fail("dropout: tensor too large");
-  if (vec)
-    k_dropout_rows<IN, OUT, RES, true><<<(uint32_t)grid, kThreads, 0, stream>>>(k);
-  else
-    k_dropout_rows<IN, OUT, RES, false><<<(uint32_t)grid, kThreads, 0, stream>>>(k);
+  k_dropout_rows<IN, OUT, RES><<<(uint32_t)grid, kThreads, 0, stream>>>(k);
   TPI_HIP(hipGetLastError());
   return 0;
 }
 
 template <int IN, int OUT>
 int launch(const tpi_dropout_args& a, hipStream_t s) {
-  return a.residual ? launch<IN, OUT, true>(a, s) : launch<IN, OUT, false>(a, s);
+  if (!a.residual) return launch<IN, OUT, false>(a, s);
+  // the residual stream and its gradient may be wider than the activations, not narrower
+  if constexpr (OUT == IN || OUT == TPI_F32) return launch<IN, OUT, true>(a, s);
+  return tpi_fail("dropout: unsupported types");
 }
 
 }  // namespace
@@ -202,7 +255,6 @@ extern "C" int tpi_dropout(const tpi_dropout_args* args, uint64_t stream) {
     if (a.sizes[d] < 1) return tpi_fail("dropout: empty dimension");
   if (a.threshold > 1ull << 32) return tpi_fail("dropout: bad threshold");
   hipStream_t s = (hipStream_t)stream;
-  // the residual stream and its gradient may be wider than the activations
   switch (a.in_type * 3 + a.out_type) {
     case TPI_F32 * 3 + TPI_F32: return launch<TPI_F32, TPI_F32>(a, s);
     case TPI_F16 * 3 + TPI_F16: return launch<TPI_F16, TPI_F16>(a, s);

@@ -27,10 +27,10 @@ namespace {
 
 constexpr int kBlock = 256;   // threads that move bytes
 constexpr int kPlan = 1024;   // threads of the one-workgroup kernels
+constexpr int kSpread = 256 * 32;  // workgroups that take pages of an unknown number
 constexpr int kRowSpan = 1024;  // table entries of a row that one workgroup of k_fork takes
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // scratch: [pages] x 4, [slots] x 5
 __device__ static inline int32_t* list(const tpi_pages& p, int i) {
@@ -56,82 +56,78 @@ __device__ static inline int32_t pages_of(int64_t tokens, int32_t per) {
 
 // ---- moving bytes ------------------------------------------------------------------------------
 
-// The tensor of chunk c of a page (chunk0 ascends).
-__device__ static inline const tpi_page_tensor& tensor_of(const tpi_pages& p, uint32_t c) {
-  int lo = 0, hi = p.ntensors - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.tensors[mid].chunk0 <= c) lo = mid; else hi = mid - 1;
+// A unit is one 16-byte access of any alignment (the GPU's need none).  A run whose bytes are no
+// multiple of 16 ends with a unit that begins 16 bytes before its end, so two units write the
+// same bytes there; one of less than 16 bytes moves byte by byte.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
+struct Unit {
+  int64_t at;      // byte offset from the chunk's base
+  uint32_t bytes;  // 16, less in a short run, 0: behind the chunk's end
+};
+
+__device__ static inline Unit unit_of(const tpi_page_chunk& c, uint32_t u) {
+  uint32_t row = 0, col = u;
+  if (c.rows > 1) {
+    row = u / c.row_units;
+    col = u - row * c.row_units;
   }
-  return p.tensors[lo];
+  if (row >= c.rows || col >= c.row_units) return Unit{0, 0};
+  const int64_t base = (int64_t)row * c.row_stride;
+  if (c.row_bytes < 16) return Unit{base, c.row_bytes};
+  const uint32_t at = col * 16, last = c.row_bytes - 16;
+  return Unit{base + (at < last ? at : last), 16};
 }
 
-template <typename T, typename F>
-__device__ static inline void over_chunk(const tpi_page_tensor& t, uint32_t chunk, F f) {
-  const uint64_t total = (uint64_t)t.rows * t.row_units;
+constexpr int kUnits = TPI_PAGE_UNITS / kBlock;  // of a thread
+
+// All of a thread's loads first, then its stores: 16 KB of a workgroup in flight.  Measured with
+// 1024 pages of 32 KB in 16 tensors: 214 us (5.0 TB/s, what a large copy reaches), 290 with half
+// of it and a lookup of the tensor before the first load.  Nontemporal stores leave the caches to
+// the pages that are read: 256 MB of 16 KB pages 36 us instead of 39.
+__device__ static inline void copy_chunk(const tpi_page_chunk& c, int64_t src, int64_t dst) {
+  const uint8_t* s = (const uint8_t*)c.base + src * c.page_stride;
+  uint8_t* d = (uint8_t*)c.base + dst * c.page_stride;
+  Unit unit[kUnits];
+  u32x4 v[kUnits];
 #pragma unroll
-  for (int k = 0; k < TPI_PAGE_UNITS / kBlock; ++k) {
-    const uint64_t u = (uint64_t)chunk * TPI_PAGE_UNITS + k * kBlock + threadIdx.x;
-    if (u >= total) continue;
-    uint64_t row = 0, col = u;
-    if (t.rows > 1) {
-      row = u / t.row_units;
-      col = u - row * t.row_units;
+  for (int k = 0; k < kUnits; ++k) {
+    unit[k] = unit_of(c, k * kBlock + threadIdx.x);
+    if (unit[k].bytes == 16) v[k] = *(const u32x4_any*)(s + unit[k].at);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    if (unit[k].bytes == 16) {
+      __builtin_nontemporal_store(v[k], (u32x4_any*)(d + unit[k].at));
+    } else {
+      for (uint32_t b = 0; b < unit[k].bytes; ++b) d[unit[k].at + b] = s[unit[k].at + b];
     }
-    f((int64_t)row * t.row_stride + (int64_t)col * (int64_t)sizeof(T));
   }
 }
 
-template <typename T>
-__device__ static inline void copy_units(const tpi_page_tensor& t, uint32_t chunk, int64_t src,
-                                         int64_t dst) {
-  const uint8_t* s = (const uint8_t*)t.base + src * t.page_stride;
-  uint8_t* d = (uint8_t*)t.base + dst * t.page_stride;
-  over_chunk<T>(t, chunk, [&](int64_t at) { *(T*)(d + at) = *(const T*)(s + at); });
-}
-
-template <typename T>
-__device__ static inline void zero_units(const tpi_page_tensor& t, uint32_t chunk, int64_t page) {
-  uint8_t* d = (uint8_t*)t.base + page * t.page_stride;
-  over_chunk<T>(t, chunk, [&](int64_t at) { *(T*)(d + at) = T{}; });
-}
-
-// Chunk c (over all tensors) of a page.
-__device__ static void copy_chunk(const tpi_pages& p, uint32_t c, int64_t src, int64_t dst) {
-  const tpi_page_tensor& t = tensor_of(p, c);
-  const uint32_t chunk = c - t.chunk0;
-  switch (t.unit) {
-    case 16: copy_units<u32x4>(t, chunk, src, dst); break;
-    case 8: copy_units<u32x2>(t, chunk, src, dst); break;
-    case 4: copy_units<uint32_t>(t, chunk, src, dst); break;
-    case 2: copy_units<uint16_t>(t, chunk, src, dst); break;
-    default: copy_units<uint8_t>(t, chunk, src, dst); break;
+__device__ static inline void zero_chunk(const tpi_page_chunk& c, int64_t page) {
+  uint8_t* d = (uint8_t*)c.base + page * c.page_stride;
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    const Unit unit = unit_of(c, k * kBlock + threadIdx.x);
+    if (unit.bytes == 16) {
+      *(u32x4_any*)(d + unit.at) = u32x4{0, 0, 0, 0};
+    } else {
+      for (uint32_t b = 0; b < unit.bytes; ++b) d[unit.at + b] = 0;
+    }
   }
 }
 
-__device__ static void zero_chunk(const tpi_pages& p, uint32_t c, int64_t page) {
-  const tpi_page_tensor& t = tensor_of(p, c);
-  const uint32_t chunk = c - t.chunk0;
-  switch (t.unit) {
-    case 16: zero_units<u32x4>(t, chunk, page); break;
-    case 8: zero_units<u32x2>(t, chunk, page); break;
-    case 4: zero_units<uint32_t>(t, chunk, page); break;
-    case 2: zero_units<uint16_t>(t, chunk, page); break;
-    default: zero_units<uint8_t>(t, chunk, page); break;
-  }
-}
-
+// Workgroups (chunk, pair): nothing to look up or divide before the first load.
 __global__ __launch_bounds__(kBlock) void k_copy(tpi_pages p, const void* src, const void* dst,
                                                  int64_t n, bool wide) {
-  const int64_t work = n * p.chunks;
-  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int64_t i = w / p.chunks;
+  for (int64_t i = blockIdx.y; i < n; i += gridDim.y) {
     const int64_t s = number(src, i, wide), d = number(dst, i, wide);
     if (s < 0 || s >= p.pages || d < 0 || d >= p.pages) {
       if (threadIdx.x == 0) refuse(p, TPI_PAGES_EPAGE);
       continue;
     }
-    copy_chunk(p, (uint32_t)(w - i * p.chunks), s, d);
+    copy_chunk(p.chunk[blockIdx.x], s, d);
   }
 }
 
@@ -160,17 +156,34 @@ __device__ static inline int scan(int v, int* total) {
   return before + x - v;
 }
 
-// Numbers of the set bits of `bits` (page 32 w + bit) that have rank lo, lo + 1, ... below
-// `limit`, in ascending order; returns the bits that were taken.
-__device__ static inline uint32_t emit(uint32_t bits, int w, int lo, int limit, int32_t* out) {
-  uint32_t taken = 0;
-  while (bits && lo < limit) {
-    const int b = __ffs(bits) - 1;
-    out[lo++] = 32 * w + b;
-    taken |= 1u << b;
-    bits &= bits - 1;
+// A pass of the workgroup over kPlan words of bits: thread t has `bits` of word base + t, whose
+// first set bit has rank `rank`.  Writes the numbers of the set bits with ranks below `limit` to
+// out[rank].  A thread per bit, 32 words apart (one per word would store up to 32 numbers one
+// after the other: 10 us of a compaction's plan instead of 6).
+struct Words {
+  uint32_t bits[kPlan];
+  int rank[kPlan];
+};
+
+__device__ static inline void emit(Words& lds, uint32_t bits, int rank, int base, int words,
+                                   int limit, int32_t* out) {
+  __syncthreads();  // the last pass has been read
+  lds.bits[threadIdx.x] = bits;
+  lds.rank[threadIdx.x] = rank;
+  __syncthreads();
+  const int n = 32 * (words - base < kPlan ? words - base : kPlan);
+  for (int i = threadIdx.x; i < n; i += kPlan) {
+    const uint32_t w = lds.bits[i >> 5], bit = 1u << (i & 31);
+    if (!(w & bit)) continue;
+    const int r = lds.rank[i >> 5] + __popc(w & (bit - 1));
+    if (r < limit) out[r] = 32 * base + i;
   }
-  return taken;
+}
+
+// `bits` without its lowest n set ones.
+__device__ static inline uint32_t without_lowest(uint32_t bits, int n) {
+  for (; n > 0 && bits; --n) bits &= bits - 1;
+  return bits;
 }
 
 // Pages of slot entry i that a fork / an extension takes.
@@ -187,6 +200,7 @@ __global__ __launch_bounds__(kPlan) void k_reserve(tpi_pages p, const void* a, c
                                                    bool more_wide, int64_t each) {
   __shared__ int s_error;
   __shared__ unsigned long long s_total;
+  __shared__ Words lds;
   const int tid = threadIdx.x;
   int32_t* mark = slot_list(p, MARK);
   int32_t* offset = slot_list(p, OFFSET);
@@ -260,7 +274,8 @@ __global__ __launch_bounds__(kPlan) void k_reserve(tpi_pages p, const void* a, c
     const int w = base + tid;
     const uint32_t bits = w < words ? p.free_bits[w] : 0;
     const int rank = found + scan(__popc(bits), &sum);
-    if (bits && rank < total) p.free_bits[w] = bits & ~emit(bits, w, rank, total, list(p, TAKEN));
+    if (bits && rank < total) p.free_bits[w] = without_lowest(bits, total - rank);
+    emit(lds, bits, rank, base, words, total, list(p, TAKEN));
     found += sum;
   }
   __syncthreads();
@@ -301,23 +316,23 @@ __global__ __launch_bounds__(kPlan) void k_reserve(tpi_pages p, const void* a, c
   if (tid == 0) p.header[TPI_PAGES_FREE] -= total;
 }
 
-// Workgroups of one entry: `spans` for its table row, then p.chunks for its partial page.
+// Workgroups (j, entry): the first `spans` of an entry take its table row, the others a chunk of
+// its partial page each.
 __global__ __launch_bounds__(kBlock) void k_fork(tpi_pages p, const void* src, const void* dst,
                                                  int64_t n, bool wide, int spans) {
-  const int64_t per = spans + p.chunks, work = n * per;
-  for (int64_t g = blockIdx.x; g < work; g += gridDim.x) {
-    const int64_t i = g / per, j = g - i * per;
+  const int j = blockIdx.x;
+  for (int64_t i = blockIdx.y; i < n; i += gridDim.y) {
     const int32_t len = slot_list(p, LENGTH)[i];
     if (len < 0) return;  // refused
     const int32_t from = slot_list(p, PAIR_SRC)[i], to = slot_list(p, PAIR_DST)[i];
     if (j >= spans) {
-      if (from >= 0 && from < p.pages && to >= 0)
-        copy_chunk(p, (uint32_t)(j - spans), from, to);
+      if (from >= 0 && from < p.pages && to >= 0) copy_chunk(p.chunk[j - spans], from, to);
       continue;
     }
     const int64_t s = number(src, i, wide), d = number(dst, i, wide);
     const int32_t full = len / p.tokens;
-    for (int64_t k = j * kRowSpan + threadIdx.x; k < (j + 1) * kRowSpan && k < full; k += kBlock) {
+    for (int64_t k = (int64_t)j * kRowSpan + threadIdx.x; k < (j + 1ll) * kRowSpan && k < full;
+         k += kBlock) {
       const int32_t page = p.table[s * p.width + k];
       p.table[d * p.width + k] = page;
       if (page >= 0 && page < p.pages) atomicAdd(&p.refs[page], 1);
@@ -373,22 +388,34 @@ __device__ static inline uint32_t bits_below(int w, int page) {
 }
 
 __global__ __launch_bounds__(kPlan) void k_plan(tpi_pages p, bool clear) {
+  __shared__ Words lds;
   const int tid = threadIdx.x;
   const int live = p.pages - p.header[TPI_PAGES_FREE];
   const int words = (p.pages + 31) / 32;
-  int holes = 0, movers = 0;
+  int holes = 0, movers = 0, clears = 0;
   for (int base = 0; base < words; base += kPlan) {
     int sum;
     const int w = base + tid;
-    const uint32_t free = w < words ? p.free_bits[w] : 0;
-    const uint32_t low = bits_below(w, live), all = bits_below(w, p.pages);
-    const uint32_t hole = free & low, mover = ~free & all & ~low;
-    const int h = scan(__popc(hole), &sum);
-    emit(hole, w, holes + h, p.pages, list(p, HOLES));
-    holes += sum;
-    const int m = scan(__popc(mover), &sum);
-    emit(mover, w, movers + m, p.pages, list(p, MOVERS));
-    movers += sum;
+    uint32_t hole = 0, mover = 0, stale = 0;
+    if (w < words) {
+      const uint32_t free = p.free_bits[w], low = bits_below(w, live);
+      const uint32_t freed = bits_below(w, p.pages) & ~low;  // the free pages afterwards
+      hole = free & low;
+      mover = ~free & freed;
+      stale = (p.stale_bits[w] | mover) & freed;  // a mover's old page is stale
+      p.free_bits[w] = freed;
+      p.stale_bits[w] = clear ? 0 : stale;
+    }
+    // both counts of a pass (at most 32 kPlan = 32768) in one sum
+    const uint32_t before = scan(__popc(hole) | __popc(mover) << 16, &sum);
+    emit(lds, hole, holes + (int)(before & 0xffff), base, words, p.pages, list(p, HOLES));
+    emit(lds, mover, movers + (int)(before >> 16), base, words, p.pages, list(p, MOVERS));
+    holes += sum & 0xffff;
+    movers += (uint32_t)sum >> 16;
+    if (!clear) continue;
+    const int c = scan(__popc(stale), &sum);
+    emit(lds, stale, clears + c, base, words, p.pages, list(p, CLEARS));
+    clears += sum;
   }
   __syncthreads();
   // as many holes below `live` as live pages at or above it, if the counts are in order
@@ -399,22 +426,6 @@ __global__ __launch_bounds__(kPlan) void k_plan(tpi_pages p, bool clear) {
     p.refs[from] = 0;
     list(p, MAP)[from] = to;
   }
-  int clears = 0;
-  for (int base = 0; base < words; base += kPlan) {
-    int sum;
-    const int w = base + tid;
-    uint32_t stale = 0;
-    if (w < words) {
-      const uint32_t freed = bits_below(w, p.pages) & ~bits_below(w, live);
-      stale = (p.stale_bits[w] | ~p.free_bits[w]) & freed;  // a mover's old page is stale
-      p.free_bits[w] = freed;
-      p.stale_bits[w] = clear ? 0 : stale;
-    }
-    if (!clear) continue;
-    const int c = scan(__popc(stale), &sum);
-    emit(stale, w, clears + c, p.pages, list(p, CLEARS));
-    clears += sum;
-  }
   if (tid == 0) {
     p.header[TPI_PAGES_LIVE] = live;
     p.header[TPI_PAGES_MOVES] = moves;
@@ -422,37 +433,44 @@ __global__ __launch_bounds__(kPlan) void k_plan(tpi_pages p, bool clear) {
   }
 }
 
-// The first `spans` workgroups take the table, the others the moved pages.
+// Workgroups (x, chunk): neighbours take neighbouring pages of one tensor, so that reads and
+// writes run through it (with neighbours in different tensors, COMPACTFIG).  The first `spans`
+// of every chunk take the table, the others the moved pages x - spans, x - spans + their number, ...
 __global__ __launch_bounds__(kBlock) void k_compact(tpi_pages p, int spans) {
-  const int live = p.header[TPI_PAGES_LIVE];
-  if ((int)blockIdx.x < spans) {
+  const int x = blockIdx.x;
+  if (x < spans) {
+    const int live = p.header[TPI_PAGES_LIVE];
     const int64_t entries = (int64_t)p.slots * p.width;
-    for (int64_t e = (int64_t)blockIdx.x * kBlock + threadIdx.x; e < entries;
-         e += (int64_t)spans * kBlock) {
+    for (int64_t e = ((int64_t)x * gridDim.y + blockIdx.y) * kBlock + threadIdx.x; e < entries;
+         e += (int64_t)spans * gridDim.y * kBlock) {
       const int32_t page = p.table[e];
       if (page >= live && page < p.pages) p.table[e] = list(p, MAP)[page];
     }
     return;
   }
-  const int64_t work = (int64_t)p.header[TPI_PAGES_MOVES] * p.chunks;
-  for (int64_t w = blockIdx.x - spans; w < work; w += gridDim.x - spans) {
-    const int64_t i = w / p.chunks;
-    copy_chunk(p, (uint32_t)(w - i * p.chunks), list(p, MOVERS)[i], list(p, HOLES)[i]);
-  }
+  const int moves = p.header[TPI_PAGES_MOVES];
+  for (int c = blockIdx.y; c < p.chunks; c += gridDim.y)
+    for (int i = x - spans; i < moves; i += gridDim.x - spans)
+      copy_chunk(p.chunk[c], list(p, MOVERS)[i], list(p, HOLES)[i]);
 }
 
 __global__ __launch_bounds__(kBlock) void k_clear(tpi_pages p) {
-  const int64_t work = (int64_t)p.header[TPI_PAGES_CLEARS] * p.chunks;
-  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int64_t i = w / p.chunks;
-    zero_chunk(p, (uint32_t)(w - i * p.chunks), list(p, CLEARS)[i]);
-  }
+  const int clears = p.header[TPI_PAGES_CLEARS];
+  for (int c = blockIdx.y; c < p.chunks; c += gridDim.y)
+    for (int i = blockIdx.x; i < clears; i += gridDim.x)
+      zero_chunk(p.chunk[c], list(p, CLEARS)[i]);
 }
 
-constexpr int64_t kMaxGrid = 1 << 20;  // the loops over work take what a grid leaves
-constexpr int kSpread = 256 * 8;       // workgroups that fill the GPU
+constexpr int64_t kMaxY = 32768;  // of a grid; the loops over entries take the rest
 
-uint32_t grid_of(int64_t work) { return (uint32_t)(work < kMaxGrid ? work : kMaxGrid); }
+uint32_t rows_of(int64_t n) { return (uint32_t)(n < kMaxY ? n : kMaxY); }
+
+// Workgroups per chunk for an unknown number of pages: enough to fill the GPU several times, so
+// that few of them wait for a last one.
+uint32_t spread(const tpi_pages* p) {
+  const int64_t per = kSpread / p->chunks + 1;
+  return (uint32_t)(per < p->pages ? per : p->pages);
+}
 
 }  // namespace
 
@@ -461,7 +479,8 @@ extern "C" {
 int tpi_pages_copy(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
                    uint64_t stream) {
   if (n <= 0) return 0;
-  k_copy<<<grid_of(n * p->chunks), kBlock, 0, (hipStream_t)stream>>>(*p, src, dst, n, wide & 1);
+  k_copy<<<dim3(p->chunks, rows_of(n)), kBlock, 0, (hipStream_t)stream>>>(*p, src, dst, n,
+                                                                           wide & 1);
   TPI_HIP(hipGetLastError());
   return 0;
 }
@@ -474,7 +493,7 @@ int tpi_pages_fork(const tpi_pages* p, const void* src, const void* dst, int64_t
   k_reserve<true><<<1, kPlan, 0, s>>>(*p, src, dst, (int)n, wide & 1, nullptr, false, 0);
   TPI_HIP(hipGetLastError());
   const int spans = (p->width + kRowSpan - 1) / kRowSpan;
-  k_fork<<<grid_of(n * (spans + p->chunks)), kBlock, 0, s>>>(*p, src, dst, n, wide & 1, spans);
+  k_fork<<<dim3(spans + p->chunks, rows_of(n)), kBlock, 0, s>>>(*p, src, dst, n, wide & 1, spans);
   TPI_HIP(hipGetLastError());
   return 0;
 }
@@ -501,12 +520,13 @@ int tpi_pages_compact(const tpi_pages* p, int clear, uint64_t stream) {
   hipStream_t s = (hipStream_t)stream;
   k_plan<<<1, kPlan, 0, s>>>(*p, clear != 0);
   TPI_HIP(hipGetLastError());
-  const int64_t entries = (int64_t)p->slots * p->width;
-  const int spans = (int)(entries < 256ll * 1024 ? (entries + 1023) / 1024 : 256);
-  k_compact<<<spans + kSpread, kBlock, 0, s>>>(*p, spans);
+  const int64_t table = ((int64_t)p->slots * p->width + 4 * kBlock - 1) / (4 * kBlock);
+  const int chunks = (int)rows_of(p->chunks);
+  const int spans = (int)(((table < 256 ? table : 256) + chunks - 1) / chunks);
+  k_compact<<<dim3(spans + spread(p), chunks), kBlock, 0, s>>>(*p, spans);
   TPI_HIP(hipGetLastError());
   if (clear) {
-    k_clear<<<kSpread, kBlock, 0, s>>>(*p);
+    k_clear<<<dim3(spread(p), chunks), kBlock, 0, s>>>(*p);
     TPI_HIP(hipGetLastError());
   }
   return 0;

@@ -170,15 +170,16 @@ typedef struct tpi_dropout_args {
 int tpi_dropout(const tpi_dropout_args* args, uint64_t stream);
 
 // ---- Pages of a paged cache (ops/paging.py) ----------------------------------------------------
-// One tensor whose first dimension is the page: `rows` runs of `row_bytes` bytes per page.
-// Pages are moved in chunks of TPI_PAGE_UNITS units of `unit` bytes (16, 8, 4, 2 or 1: what
-// base, strides and row_bytes are multiples of); chunk0 = chunks of the tensors before it.
+// What one workgroup moves of a page: `rows` runs of `row_bytes` bytes in a tensor whose first
+// dimension is the page, at most TPI_PAGE_UNITS units of 16 bytes (of any alignment), a run
+// taking row_units = ceil(row_bytes / 16) of them.  A long run is cut into chunks of one row; a
+// piece of less than 16 bytes begins earlier, in the one before it.
 #define TPI_PAGE_UNITS 1024
-typedef struct tpi_page_tensor {
-  uint64_t base;
+typedef struct tpi_page_chunk {
+  uint64_t base;                    // of page 0
   int64_t page_stride, row_stride;  // bytes
-  uint32_t rows, row_units, unit, chunk0;
-} tpi_page_tensor;
+  uint32_t row_bytes, rows, row_units, pad_;
+} tpi_page_chunk;
 enum {  // words of the header
   TPI_PAGES_FREE = 0,    // pages without a reference
   TPI_PAGES_ERROR = 1,   // first refusal since it was last cleared, TPI_PAGES_E*
@@ -206,10 +207,8 @@ typedef struct tpi_pages {
   uint32_t* free_bits;   // [ceil(pages / 32)] 1: no reference
   uint32_t* stale_bits;  // [ceil(pages / 32)] 1: not known to be zero (free pages only)
   int32_t* scratch;      // 4 * pages + 5 * slots words
-  const tpi_page_tensor* tensors;
-  int32_t pages, slots, width, tokens;
-  int32_t ntensors;
-  int32_t chunks;        // of one page, over all tensors
+  const tpi_page_chunk* chunk;  // [chunks] of one page, over all tensors
+  int32_t pages, slots, width, tokens, chunks, pad_;
 } tpi_pages;
 // `wide` bit 0: slot / page numbers are int64, else int32; bit 1: the same of `more`.
 // copy: page src[i] to page dst[i] in every tensor; no page may be a destination twice, nor a

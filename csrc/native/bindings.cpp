@@ -179,7 +179,7 @@ PYBIND11_MODULE(_tpi_native, m) {
     return py::make_tuple(bad, first);
   });
   m.attr("PAGES_SIZE") = (int)sizeof(tpi_pages);
-  m.attr("PAGE_TENSOR_SIZE") = (int)sizeof(tpi_page_tensor);
+  m.attr("PAGE_CHUNK_SIZE") = (int)sizeof(tpi_page_chunk);
   m.def("pages_copy", [](const py::bytes& pool, uintptr_t src, uintptr_t dst, int64_t n) {
     tpi::pages_copy(struct_of<tpi_pages>(pool), (const int64_t*)src, (const int64_t*)dst, n);
   });

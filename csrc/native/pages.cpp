@@ -26,13 +26,12 @@ bool page_ok(const tpi_pages& p, int64_t s) { return s >= 0 && s < p.pages; }
 
 // Page `src` copied to page `dst` in every tensor, or `dst` cleared (src < 0).
 void move_page(const tpi_pages& p, int64_t src, int64_t dst) {
-  for (int t = 0; t < p.ntensors; ++t) {
-    const tpi_page_tensor& x = p.tensors[t];
-    const size_t bytes = (size_t)x.row_units * x.unit;
+  for (int c = 0; c < p.chunks; ++c) {
+    const tpi_page_chunk& x = p.chunk[c];
     for (uint32_t r = 0; r < x.rows; ++r) {
       uint8_t* row = (uint8_t*)x.base + (int64_t)r * x.row_stride;
-      if (src < 0) memset(row + dst * x.page_stride, 0, bytes);
-      else memcpy(row + dst * x.page_stride, row + src * x.page_stride, bytes);
+      if (src < 0) memset(row + dst * x.page_stride, 0, x.row_bytes);
+      else memcpy(row + dst * x.page_stride, row + src * x.page_stride, x.row_bytes);
     }
   }
 }

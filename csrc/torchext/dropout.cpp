@@ -38,6 +38,7 @@ void dropout_range(const tpi_dropout_args& a, uint64_t seed, uint64_t draw, uint
     index[d] = (int64_t)(rest % (uint64_t)a.sizes[d]);
     rest /= (uint64_t)a.sizes[d];
   }
+  const tpi_keep keep = tpi_keep_below(a.threshold);
   uint64_t block = ~0ull;
   uint32_t kept = 0;
   for (uint64_t e = lo; e < hi; ++e) {
@@ -51,7 +52,7 @@ void dropout_range(const tpi_dropout_args& a, uint64_t seed, uint64_t draw, uint
     }
     if (n >> 3 != block) {
       block = n >> 3;
-      kept = tpi_draw_block(block, draw, seed, a.threshold);
+      kept = tpi_draw_block(block, draw, seed, keep);
     }
     float v = 0.0f;
     if (kept >> (n & 7) & 1) v = load((const void*)a.x, x, a.in_type) * a.scale;

@@ -28,7 +28,8 @@ from .packing import canonical_view
 
 HEADER, CHUNK_UNITS = 16, 1024  # TPI_PAGES_HEADER, TPI_PAGE_UNITS
 _POOL = struct.Struct("<8Q6i")  # tpi_pages
-_TENSOR = struct.Struct("<Q2q4I")  # tpi_page_tensor
+_CHUNK = np.dtype([("base", "<u8"), ("page_stride", "<i8"), ("row_stride", "<i8"),  # tpi_page_chunk
+                   ("row_bytes", "<u4"), ("rows", "<u4"), ("row_units", "<u4"), ("pad", "<u4")])
 _FREE, _ERROR = 0, 1
 _ERRORS = {1: "not enough free pages", 2: "a slot is out of range",
            3: "a fork's destination holds a sequence (or is its source)",
@@ -102,14 +103,14 @@ class PagePool:
                                     device=self.device)
         at = [t.data_ptr() for t in (self._header, self.refs, self.lengths, self.table,
                                      self._free_bits, self._stale_bits, self._scratch,
-                                     self._descriptors)]
+                                     self._chunk)]
         self._args = _POOL.pack(*at, self.pages, self.slots, self.width, self.page_tokens,
-                                len(tensors), self._chunks)
+                                self._chunks, 0)
         self._write_books(np.full((self.slots, self.width), -1, np.int32),
                           np.zeros(self.slots, np.int32))
 
     def _lay_out_tensors(self) -> None:
-        rows, chunk0 = [], 0
+        parts = []
         for t in self.tensors:
             elem = t.element_size()
             strides = sorted((st, size) for st, size in zip(t.stride(), t.shape) if size > 1)
@@ -123,21 +124,37 @@ class PagePool:
                 raise ValueError("a page's bytes must be contiguous runs with one stride between "
                                  "them, not %s with strides %s" % (tuple(t.shape), t.stride()))
             runs, run_stride = dims[0] if len(dims) == 2 else (1, 0)
-            run = dims[-1][0] * elem
-            page_stride, run_stride = t.stride(0) * elem, run_stride * elem
-            unit = 16
-            while any(v % unit for v in (t.data_ptr(), page_stride, run_stride, run)):
-                unit //= 2
-            if runs >= 1 << 31 or run // unit >= 1 << 31:
-                raise ValueError("a page is too large")
-            rows.append(_TENSOR.pack(t.data_ptr(), page_stride, run_stride, runs, run // unit,
-                                     unit, chunk0))
-            chunk0 += -(-runs * (run // unit) // CHUNK_UNITS)
-        if chunk0 >= 1 << 30:
+            parts.append(self._cut(t.data_ptr(), t.stride(0) * elem, runs, run_stride * elem,
+                                   dims[-1][0] * elem))
+        chunks = np.concatenate(parts)
+        if len(chunks) >= 1 << 24:
             raise ValueError("the pages are too large")
-        self._chunks = chunk0
-        host = torch.frombuffer(bytearray(b"".join(rows)), dtype=torch.uint8)
-        self._descriptors = host.to(self.device)
+        self._chunks = len(chunks)
+        self._chunk = torch.from_numpy(chunks.view(np.uint8)).to(self.device)
+
+    @staticmethod
+    def _cut(base: int, page_stride: int, runs: int, run_stride: int, run: int) -> np.ndarray:
+        """Chunks of one tensor's page: whole runs while several fit, pieces of one otherwise."""
+        units = -(-run // 16)
+        if units <= CHUNK_UNITS:
+            step = CHUNK_UNITS // units
+            rows = np.arange(0, runs, step)
+            out = np.zeros(len(rows), _CHUNK)
+            out["base"] = base + rows * run_stride
+            out["rows"] = np.minimum(step, runs - rows)
+            out["row_bytes"], out["row_units"] = run, units
+        else:
+            step = CHUNK_UNITS * 16
+            starts = np.arange(0, run, step)
+            ends = np.minimum(starts + step, run)
+            starts = np.minimum(starts, run - 16)  # not less than one unit
+            out = np.zeros(runs * len(starts), _CHUNK)
+            out["base"] = (base + np.arange(runs)[:, None] * run_stride + starts).reshape(-1)
+            out["rows"] = 1
+            out["row_bytes"] = np.tile(ends - starts, runs)
+            out["row_units"] = (out["row_bytes"] + 15) // 16
+        out["page_stride"], out["row_stride"] = page_stride, run_stride
+        return out
 
     def _bind_meta(self, sizes: List[int], words: int) -> None:
         parts = self.meta.split(sizes)

@@ -35,7 +35,7 @@ def test_philox_known_answers():
 
 def test_argument_blocks_match_the_c_structs():
     assert paging._POOL.size == ops.native().PAGES_SIZE
-    assert paging._TENSOR.size == ops.native().PAGE_TENSOR_SIZE
+    assert paging._CHUNK.itemsize == ops.native().PAGE_CHUNK_SIZE
 
 
 @pytest.mark.parametrize("p", [0.0, 1e-9, 0.1, 0.5, 0.75, 1 - 2 ** -20, 1.0])
