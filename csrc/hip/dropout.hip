@@ -126,9 +126,9 @@ __global__ __launch_bounds__(kThreads) void k_dropout_rows(RowArgs a) {
   const uint64_t t = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
   int64_t row = 0;
   if (a.rows > 1)
-    row = t >> 31 ? (int64_t)(t / a.per_row)
-                  : (int64_t)((__umulhi((uint32_t)t, a.by_row.mul) + (uint32_t)t) >>
-                              a.by_row.shift);
+    row = (t | a.per_row) >> 31 ? (int64_t)(t / a.per_row)
+                                : (int64_t)((__umulhi((uint32_t)t, a.by_row.mul) + (uint32_t)t) >>
+                                            a.by_row.shift);
   if (row >= a.rows) return;
   const uint64_t b = t - (uint64_t)row * a.per_row;
   const uint64_t start = a.first + (uint64_t)row * (uint64_t)a.si, block = (start >> 3) + b;
@@ -232,7 +232,8 @@ int launch(const tpi_dropout_args& a, hipStream_t stream) {
   }
   const uint64_t blocks = k.per_row * (uint64_t)k.rows;
   const uint64_t grid = (blocks + kThreads - 1) / kThreads;
-  if (grid > 0x7fffffffull) return tpi_fail("dropout: tensor too large");
+  // a launch has fewer than 2^32 threads: 34e9 elements
+  if (grid * kThreads >> 32) return tpi_fail("dropout: tensor too large");
   k_dropout_rows<IN, OUT, RES><<<(uint32_t)grid, kThreads, 0, stream>>>(k);
   TPI_HIP(hipGetLastError());
   return 0;

@@ -10,7 +10,7 @@
 // reference counts and bits are changed by integer atomics only, so that every result is the same
 // on every run -- and on the host implementation (csrc/native/pages.cpp).
 //
-//  k_reserve      one workgroup: checks a fork or an extension as a whole, then takes its pages
+//  k_reserve(_few)  one workgroup: checks a fork or an extension as a whole, then takes its pages
 //                 from the free bits (1024 words at a time: popcount, prefix sum)
 //  k_fork         table rows of the forks, and their partial pages' bytes
 //  k_free         a workgroup per slot
@@ -316,6 +316,117 @@ __global__ __launch_bounds__(kPlan) void k_reserve(tpi_pages p, const void* a, c
   if (tid == 0) p.header[TPI_PAGES_FREE] -= total;
 }
 
+// k_reserve for few entries in a pool of ordinary size: an entry stays in its thread's registers,
+// slots named twice are found in a bitmap in LDS, and the pages taken stay there too, so that three
+// loads follow one another instead of nine: 128 forks 5.6 us instead of 7.3, 192 extensions 5.8
+// instead of 8.1.
+constexpr int kFewSlots = 1 << 16, kFewPages = 1 << 20, kFewTaken = 4096;
+
+template <bool FORK>
+__global__ __launch_bounds__(kPlan) void k_reserve_few(tpi_pages p, const void* a, const void* b,
+                                                       int n, bool wide, const void* more,
+                                                       bool more_wide, int64_t each) {
+  __shared__ Words lds;
+  __shared__ uint32_t s_seen[kFewSlots / 32];
+  __shared__ int32_t s_taken[kFewTaken], s_offset[kPlan];
+  __shared__ int64_t s_row[kPlan];
+  __shared__ int s_error, s_twice, s_most;
+  const int tid = threadIdx.x, words = (p.pages + 31) / 32;
+  const int64_t s = tid < n ? number(a, tid, wide) : 0;
+  const int64_t d = FORK && tid < n ? number(b, tid, wide) : s;
+  uint32_t bits = tid < words ? p.free_bits[tid] : 0;
+  const int free = p.header[TPI_PAGES_FREE];
+  for (int i = tid; i < (p.slots + 31) / 32; i += kPlan) s_seen[i] = 0;
+  if (tid == 0) s_error = s_twice = s_most = 0;
+  const bool mine = tid < n && s >= 0 && s < p.slots && d >= 0 && d < p.slots;
+  int error = tid < n && !mine ? TPI_PAGES_ESLOT : 0;
+  const int32_t old = mine ? p.lengths[s] : 0;
+  int64_t len = old;
+  if (mine && FORK) {
+    if (s == d || p.lengths[d] != 0) error = TPI_PAGES_EBUSY;
+  } else if (mine) {
+    const int64_t m = more ? number(more, tid, more_wide) : each;
+    if (m < 0) error = TPI_PAGES_ETOKENS;
+    else if (m > (int64_t)p.width * p.tokens - old || old + m > 0x7fffffff)
+      error = TPI_PAGES_EWIDTH;
+    else len = old + m;
+  }
+  const int32_t had = pages_of(old, p.tokens);
+  int need = !mine || error ? 0 : FORK ? old % p.tokens != 0 : pages_of(len, p.tokens) - had;
+  const bool full = need > free;  // and their sum stays below 2^31 without such
+  if (full) need = 0;
+  int32_t from = -1;
+  if (FORK && need) from = p.table[s * p.width + old / p.tokens];
+  __syncthreads();
+  if (mine && (atomicOr(&s_seen[d >> 5], 1u << (d & 31)) >> (d & 31) & 1)) s_twice = 1;
+  if (error) atomicMax(&s_error, error);
+  if (need > 1) atomicMax(&s_most, need);
+  int total;
+  const int offset = scan(need, &total);  // (its barriers order the shared words, too)
+  if (full) atomicMax(&s_error, TPI_PAGES_ENOSPACE);
+  __syncthreads();
+  const int why = s_error > TPI_PAGES_ENOSPACE ? s_error : s_twice ? TPI_PAGES_EDUPLICATE
+                  : s_error || total > free ? TPI_PAGES_ENOSPACE : 0;
+  if (why) {
+    if (tid == 0) refuse(p, why);
+    if (FORK && tid < n) slot_list(p, LENGTH)[tid] = -1;  // nothing for k_fork
+    return;
+  }
+  const bool near = total <= kFewTaken;
+  int found = 0;
+  for (int base = 0; base < words && found < total; base += kPlan) {
+    int sum;
+    const int w = base + tid;
+    if (base) bits = w < words ? p.free_bits[w] : 0;
+    const int rank = found + scan(__popc(bits), &sum);
+    if (bits && rank < total) p.free_bits[w] = without_lowest(bits, total - rank);
+    if (near) emit(lds, bits, rank, base, words, total, s_taken);
+    else emit(lds, bits, rank, base, words, total, list(p, TAKEN));
+    found += sum;
+  }
+  if (!FORK) {
+    s_offset[tid] = tid < n ? offset : total;
+    s_row[tid] = s * p.width + had;
+  }
+  __syncthreads();
+  if (found < total) {
+    if (tid == 0) refuse(p, TPI_PAGES_ESTATE);
+    if (FORK && tid < n) slot_list(p, LENGTH)[tid] = -1;
+    return;
+  }
+  const int32_t* far = list(p, TAKEN);
+  if (FORK) {
+    if (tid < n) {
+      const int32_t to = need ? near ? s_taken[offset] : far[offset] : -1;
+      slot_list(p, LENGTH)[tid] = old;
+      slot_list(p, PAIR_SRC)[tid] = from;
+      slot_list(p, PAIR_DST)[tid] = to;
+      if (need) p.refs[to] = 1;
+    }
+  } else {
+    if (s_most <= 1) {
+      if (need) {
+        const int32_t page = near ? s_taken[offset] : far[offset];
+        p.table[s * p.width + had] = page;
+        p.refs[page] = 1;
+      }
+    } else {
+      for (int r = tid; r < total; r += kPlan) {
+        int lo = 0, hi = n - 1;  // the last entry that begins at or before r
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (s_offset[mid] <= r) lo = mid; else hi = mid - 1;
+        }
+        const int32_t page = near ? s_taken[r] : far[r];
+        p.table[s_row[lo] + (r - s_offset[lo])] = page;
+        p.refs[page] = 1;
+      }
+    }
+    if (tid < n) p.lengths[s] = (int32_t)len;
+  }
+  if (tid == 0) p.header[TPI_PAGES_FREE] = free - total;
+}
+
 // Workgroups (j, entry): the first `spans` of an entry take its table row, the others a chunk of
 // its partial page each.
 __global__ __launch_bounds__(kBlock) void k_fork(tpi_pages p, const void* src, const void* dst,
@@ -344,18 +455,33 @@ __global__ __launch_bounds__(kBlock) void k_fork(tpi_pages p, const void* src, c
   }
 }
 
-__global__ __launch_bounds__(kBlock) void k_free(tpi_pages p, const void* slots, int64_t n,
-                                                 bool wide) {
-  __shared__ int s_bad, s_len, s_count;
-  if (threadIdx.x == 0) {
-    s_bad = 0;
-    s_count = 0;
-  }
+// A free of many slots: whether one is out of range, for all of k_free's workgroups.
+__global__ __launch_bounds__(kPlan) void k_free_check(tpi_pages p, const void* slots, int64_t n,
+                                                      bool wide) {
+  __shared__ int s_bad;
+  if (threadIdx.x == 0) s_bad = 0;
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < n; i += kBlock) {  // every workgroup comes to the same end
+  for (int64_t i = threadIdx.x; i < n; i += kPlan) {
     const int64_t s = number(slots, i, wide);
     if (s < 0 || s >= p.slots) s_bad = 1;
   }
+  __syncthreads();
+  if (threadIdx.x == 0) p.header[TPI_PAGES_BAD] = s_bad;
+}
+
+__global__ __launch_bounds__(kBlock) void k_free(tpi_pages p, const void* slots, int64_t n,
+                                                 bool wide, bool checked) {
+  __shared__ int s_bad, s_len, s_count;
+  if (threadIdx.x == 0) {
+    s_bad = checked ? p.header[TPI_PAGES_BAD] : 0;
+    s_count = 0;
+  }
+  __syncthreads();
+  if (!checked)
+    for (int64_t i = threadIdx.x; i < n; i += kBlock) {  // every workgroup comes to the same end
+      const int64_t s = number(slots, i, wide);
+      if (s < 0 || s >= p.slots) s_bad = 1;
+    }
   __syncthreads();
   if (s_bad) {
     if (threadIdx.x == 0) refuse(p, TPI_PAGES_ESLOT);
@@ -434,7 +560,7 @@ __global__ __launch_bounds__(kPlan) void k_plan(tpi_pages p, bool clear) {
 }
 
 // Workgroups (x, chunk): neighbours take neighbouring pages of one tensor, so that reads and
-// writes run through it (with neighbours in different tensors, COMPACTFIG).  The first `spans`
+// writes run through it (neighbours in different tensors measure the same).  The first `spans`
 // of every chunk take the table, the others the moved pages x - spans, x - spans + their number, ...
 __global__ __launch_bounds__(kBlock) void k_compact(tpi_pages p, int spans) {
   const int x = blockIdx.x;
@@ -472,6 +598,10 @@ uint32_t spread(const tpi_pages* p) {
   return (uint32_t)(per < p->pages ? per : p->pages);
 }
 
+bool few(const tpi_pages* p, int64_t n) {
+  return n <= kPlan && p->slots <= kFewSlots && p->pages <= kFewPages;
+}
+
 }  // namespace
 
 extern "C" {
@@ -490,7 +620,8 @@ int tpi_pages_fork(const tpi_pages* p, const void* src, const void* dst, int64_t
   if (n <= 0) return 0;
   if (n > p->slots) return tpi_fail("fork: more destinations than slots");
   hipStream_t s = (hipStream_t)stream;
-  k_reserve<true><<<1, kPlan, 0, s>>>(*p, src, dst, (int)n, wide & 1, nullptr, false, 0);
+  const auto reserve = few(p, n) ? k_reserve_few<true> : k_reserve<true>;
+  reserve<<<1, kPlan, 0, s>>>(*p, src, dst, (int)n, wide & 1, nullptr, false, 0);
   TPI_HIP(hipGetLastError());
   const int spans = (p->width + kRowSpan - 1) / kRowSpan;
   k_fork<<<dim3(spans + p->chunks, rows_of(n)), kBlock, 0, s>>>(*p, src, dst, n, wide & 1, spans);
@@ -502,8 +633,9 @@ int tpi_pages_extend(const tpi_pages* p, const void* slots, int64_t n, int wide,
                      const void* more, int64_t each, uint64_t stream) {
   if (n <= 0) return 0;
   if (n > p->slots) return tpi_fail("extend: more sequences than slots");
-  k_reserve<false><<<1, kPlan, 0, (hipStream_t)stream>>>(*p, slots, nullptr, (int)n, wide & 1,
-                                                         more, (wide & 2) != 0, each);
+  const auto reserve = few(p, n) ? k_reserve_few<false> : k_reserve<false>;
+  reserve<<<1, kPlan, 0, (hipStream_t)stream>>>(*p, slots, nullptr, (int)n, wide & 1, more,
+                                                (wide & 2) != 0, each);
   TPI_HIP(hipGetLastError());
   return 0;
 }
@@ -511,7 +643,13 @@ int tpi_pages_extend(const tpi_pages* p, const void* slots, int64_t n, int wide,
 int tpi_pages_free(const tpi_pages* p, const void* slots, int64_t n, int wide, uint64_t stream) {
   if (n <= 0) return 0;
   if (n > p->slots) return tpi_fail("free: more sequences than slots");
-  k_free<<<(uint32_t)n, kBlock, 0, (hipStream_t)stream>>>(*p, slots, n, wide & 1);
+  hipStream_t s = (hipStream_t)stream;
+  const bool many = n > kPlan;  // up to here a workgroup's own look at all slots is 4 loads a thread
+  if (many) {
+    k_free_check<<<1, kPlan, 0, s>>>(*p, slots, n, wide & 1);
+    TPI_HIP(hipGetLastError());
+  }
+  k_free<<<(uint32_t)n, kBlock, 0, s>>>(*p, slots, n, wide & 1, many);
   TPI_HIP(hipGetLastError());
   return 0;
 }

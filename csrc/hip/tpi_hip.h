@@ -186,6 +186,8 @@ enum {  // words of the header
   TPI_PAGES_LIVE = 2,    // scratch of a compaction: live pages, pages to move, pages to clear
   TPI_PAGES_MOVES = 3,
   TPI_PAGES_CLEARS = 4,
+  TPI_PAGES_BAD = 5,     // scratch of a free: some slot is out of range
+  TPI_PAGES_SHAPE = 8,   // pages, slots, width, tokens: whose books these are
   TPI_PAGES_HEADER = 16
 };
 enum {

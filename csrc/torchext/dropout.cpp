@@ -128,6 +128,8 @@ at::Tensor dropout_pass(const at::Tensor& x, const at::Tensor& residual, at::Sca
   at::Tensor out = at::empty_like(residual.defined() ? residual : x, x.options().dtype(out_type));
   const int64_t n = x.numel();
   if (n == 0) return out;  // nor will the backward pass read `used`
+  TORCH_CHECK(!x._is_zerotensor() && !(residual.defined() && residual._is_zerotensor()),
+              "dropout of a tensor without storage");
   tpi_dropout_args a{};
   a.x = (uint64_t)x.const_data_ptr();
   a.residual = residual.defined() ? (uint64_t)residual.const_data_ptr() : 0;
@@ -202,7 +204,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     const at::Tensor& grad = grads[0];
     at::Tensor dx, dr;
     if (grad.defined() && ctx->saved_data["x"].toBool())
-      dx = run(grad, at::Tensor(), (at::ScalarType)ctx->saved_data["type"].toInt(),
+      dx = run(grad.resolve_neg(), at::Tensor(), (at::ScalarType)ctx->saved_data["type"].toInt(),
                c10::static_intrusive_pointer_cast<Mask>(ctx->saved_data["mask"].toCapsule()));
     if (ctx->saved_data["residual"].toBool()) dr = grad;
     return {dx, dr, at::Tensor(), at::Tensor()};
@@ -230,7 +232,8 @@ at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residua
   mask->scale = (float)scale;
   mask->strides = std::move(strides);
   if (state) mask->state = *state;
-  return run(x, residual ? *residual : at::Tensor(),
+  // views that are negated lazily (the imaginary part of a conjugate) are written out
+  return run(x.resolve_neg(), residual ? residual->resolve_neg() : at::Tensor(),
              residual ? residual->scalar_type() : x.scalar_type(), mask);
 }
 

@@ -446,6 +446,8 @@ class TrainingState:
         for name, saved in (state.get("stateful") or {}).items():
             if name in self.stateful:
                 self.stateful[name].load_state_dict(from_jsonable(saved))
+        for pool in self.paged.values():
+            pool.check()
 
     def resume(self, persist_path: Optional[str] = None) -> Optional[Dict]:
         """Restore device tensors (host region, else ``persist_path``) and host tensors;

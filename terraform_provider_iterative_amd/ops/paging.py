@@ -30,7 +30,7 @@ HEADER, CHUNK_UNITS = 16, 1024  # TPI_PAGES_HEADER, TPI_PAGE_UNITS
 _POOL = struct.Struct("<8Q6i")  # tpi_pages
 _CHUNK = np.dtype([("base", "<u8"), ("page_stride", "<i8"), ("row_stride", "<i8"),  # tpi_page_chunk
                    ("row_bytes", "<u4"), ("rows", "<u4"), ("row_units", "<u4"), ("pad", "<u4")])
-_FREE, _ERROR = 0, 1
+_FREE, _ERROR, _SHAPE = 0, 1, 8  # words of the header
 _ERRORS = {1: "not enough free pages", 2: "a slot is out of range",
            3: "a fork's destination holds a sequence (or is its source)",
            4: "a sequence would be longer than a row of the table",
@@ -89,16 +89,18 @@ class PagePool:
             raise ValueError("page_tokens must be in [1, 2^20]")
         if self.slots < 1 or self.width < 1:
             raise ValueError("slots and width must be positive")
-        # 32-bit numbers, and a prefix of every word that one scan of the kernels can add up
-        if self.pages >= 1 << 30 or self.slots >= 1 << 30 or self.width >= 1 << 30:
+        # what one launch of the kernels can number
+        if self.pages >= 1 << 30 or self.slots >= 1 << 23 or self.width >= 1 << 30:
             raise ValueError("too many pages, slots or pages of a sequence")
+        if any(t.requires_grad for t in tensors):
+            raise ValueError("a pool's tensors are written in place: none may require a gradient")
         self.tensors = tensors
         self._lay_out_tensors()
         words = (self.pages + 31) // 32
-        sizes = [HEADER, _pad4(self.pages), _pad4(self.slots), _pad4(self.slots * self.width),
-                 _pad4(words), _pad4(words)]
-        self.meta = torch.zeros(sum(sizes), dtype=torch.int32, device=self.device)
-        self._bind_meta(sizes, words)
+        self._sizes = [HEADER, _pad4(self.pages), _pad4(self.slots), _pad4(self.slots * self.width),
+                       _pad4(words), _pad4(words)]
+        self.meta = torch.empty(sum(self._sizes), dtype=torch.int32, device=self.device)
+        self._bind_meta(words)
         self._scratch = torch.empty(4 * self.pages + 5 * self.slots, dtype=torch.int32,
                                     device=self.device)
         at = [t.data_ptr() for t in (self._header, self.refs, self.lengths, self.table,
@@ -127,7 +129,7 @@ class PagePool:
             parts.append(self._cut(t.data_ptr(), t.stride(0) * elem, runs, run_stride * elem,
                                    dims[-1][0] * elem))
         chunks = np.concatenate(parts)
-        if len(chunks) >= 1 << 24:
+        if len(chunks) >= 1 << 23:
             raise ValueError("the pages are too large")
         self._chunks = len(chunks)
         self._chunk = torch.from_numpy(chunks.view(np.uint8)).to(self.device)
@@ -156,8 +158,8 @@ class PagePool:
         out["page_stride"], out["row_stride"] = page_stride, run_stride
         return out
 
-    def _bind_meta(self, sizes: List[int], words: int) -> None:
-        parts = self.meta.split(sizes)
+    def _bind_meta(self, words: int) -> None:
+        parts = self.meta.split(self._sizes)
         self._header = parts[0]
         self.refs, self.lengths = parts[1][:self.pages], parts[2][:self.slots]
         self.table = parts[3][:self.slots * self.width].view(self.slots, self.width)
@@ -189,13 +191,15 @@ class PagePool:
         free = refs == 0
         words = self._free_bits.numel()
         packed = np.packbits(np.pad(free, (0, 32 * words - self.pages)), bitorder="little")
-        header = np.zeros(HEADER, np.int32)
+        meta = np.zeros(self.meta.numel(), np.int32)
+        header, refs_, lengths_, table_, free_, stale_ = np.split(meta, np.cumsum(self._sizes)[:-1])
         header[_FREE] = int(free.sum())
-        for part, value in ((self._header, header), (self.refs, refs.astype(np.int32)),
-                            (self.lengths, lengths), (self.table, table),
-                            (self._free_bits, packed.view(np.int32)),
-                            (self._stale_bits, packed.view(np.int32))):
-            part.copy_(torch.from_numpy(np.ascontiguousarray(value)))
+        header[_SHAPE:_SHAPE + 4] = self._shape()
+        refs_[:self.pages] = refs
+        lengths_[:self.slots] = lengths
+        table_[:table.size] = table.reshape(-1)
+        free_[:words] = stale_[:words] = packed.view(np.int32)
+        self.meta.copy_(torch.from_numpy(meta))
 
     # -- operations ---------------------------------------------------------------------------
     def _numbers(self, what: str, values: Numbers, limit: int, distinct: bool = False):
@@ -303,11 +307,18 @@ class PagePool:
         written since the last time."""
         self._enqueue("compact", int(clear) if self._on_device else bool(clear))
 
+    def _shape(self) -> List[int]:
+        return [self.pages, self.slots, self.width, self.page_tokens]
+
     # -- what the host may know ---------------------------------------------------------------
     def check(self) -> None:
-        """Raise :class:`PageError` if an operation has been refused since the last check.  Waits for
-        the device."""
-        code = int(self._header[_ERROR])
+        """Raise :class:`PageError` if an operation has been refused since the last check, or the
+        books are not this pool's (of a checkpoint of another one).  Waits for the device."""
+        header = self._header.tolist()
+        if header[_SHAPE:_SHAPE + 4] != self._shape():
+            raise PageError("the books are those of a pool of %d pages, %d slots of %d pages and %d "
+                            "tokens a page" % tuple(header[_SHAPE:_SHAPE + 4]))
+        code = header[_ERROR]
         if code:
             self._header[_ERROR] = 0
             raise PageError(_ERRORS.get(code, "error %d" % code))

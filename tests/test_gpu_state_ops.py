@@ -99,6 +99,16 @@ def test_dropout_of_views(view, dtype):
     _same(grad, ops.dropout(torch.ones(host.shape, dtype=dtype), 0.4, (2, 3)))
 
 
+def test_the_gradient_of_an_expanded_residual_is_summed():
+    x = _randn((6, 32, 64), torch.float32, 1).cuda().requires_grad_(True)
+    r = _randn((64,), torch.float32, 2).cuda().requires_grad_(True)
+    out = ops.dropout(x, 0.3, (1, 2), residual=r.expand(6, 32, 64))
+    grad = torch.randint(-8, 9, out.shape, device="cuda").float()  # their sums are exact
+    dx, dr = torch.autograd.grad(out, (x, r), grad)
+    assert torch.equal(dr, grad.sum((0, 1)))
+    _same(dx, ops.dropout(grad.cpu(), 0.3, (1, 2)))
+
+
 @pytest.mark.parametrize("starts,shape", [((0, 0, 0), (4, 6, 2048)), ((1, 2, 512), (2, 3, 512)),
                                           ((1, 2, 513), (2, 3, 511)), ((3, 5, 2047), (1, 1, 1)),
                                           ((0, 1, 7), (4, 4, 1001))])
@@ -213,7 +223,7 @@ def _pools(kind, pages, tokens, slots, width, seed=0):
 
 
 def _equal(host, dev):
-    assert torch.equal(host.meta[16:], dev.meta[16:].cpu())  # books behind the header's scratch
+    assert torch.equal(host.meta[8:], dev.meta[8:].cpu())  # all but the header's scratch
     assert host.status() == dev.status()
     for a, b in zip(host.tensors, dev.tensors):
         assert torch.equal(a, b.cpu())
@@ -265,6 +275,15 @@ def test_many_slots_long_sequences_and_many_pages():
     for pool in (host, dev):
         pool.free(list(range(0, 2500, 3)))
         pool.compact(clear=True)
+    _equal(host, dev)
+    bad = torch.arange(2000, device="cuda")  # more slots than one look takes, one out of range
+    bad[1999] = 2500
+    dev.free(bad)
+    with pytest.raises(ops.PageError, match="slot is out of range"):
+        dev.check()
+    _equal(host, dev)
+    for pool in (host, dev):
+        pool.free(list(range(2000)))
     _equal(host, dev)
     with pytest.raises(ops.PageError):
         host.extend([0], 5001)

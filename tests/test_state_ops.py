@@ -140,6 +140,25 @@ def test_views_are_masked_by_their_logical_index(view):
     assert torch.equal(ops.dropout(x, 0.4, (2, 3), residual=turned), want)
 
 
+def test_lazily_negated_views():
+    z = torch.view_as_complex(torch.randn(100, 2, generator=torch.Generator().manual_seed(3)))
+    x = torch.conj(z).imag
+    assert x.is_neg()
+    want = ops.dropout(-z.imag.contiguous(), 0.3, (1, 2))
+    assert torch.equal(ops.dropout(x, 0.3, (1, 2)), want)
+    assert torch.equal(ops.dropout(torch.zeros(100), 0.3, (1, 2), residual=x), -z.imag)
+
+
+def test_the_gradient_of_an_expanded_residual_is_summed():
+    x, r = torch.randn(5, 7, requires_grad=True), torch.randn(7, requires_grad=True)
+    out = ops.dropout(x, 0.3, (1, 2), residual=r.expand(5, 7))
+    grad = torch.randint(-8, 9, (5, 7)).float()
+    dx, dr = torch.autograd.grad(out, (x, r), grad)
+    assert torch.equal(dr, grad.sum(0)) and torch.equal(dx, ops.dropout(grad, 0.3, (1, 2)))
+    same, = torch.autograd.grad(ops.dropout(x, 0.3, (1, 2), residual=x), x, grad)
+    assert torch.equal(same, dx + grad)
+
+
 @pytest.mark.parametrize("starts,shape", [((0, 0, 0), (4, 6, 33)), ((1, 2, 5), (2, 3, 17)),
                                           ((3, 5, 32), (1, 1, 1)), ((0, 0, 16), (4, 6, 8))])
 def test_a_shard_has_the_wholes_mask(starts, shape):
@@ -321,7 +340,8 @@ def test_a_pool_refuses_what_it_cannot_hold():
     for args in (([], 4, 3), ([ok, torch.zeros(9, 4)], 4, 3), ([torch.zeros(8)], 4, 3),
                  ([torch.zeros(8, 0)], 4, 3), ([ok], 0, 3), ([ok], 4, 0), ([ok], 4, 3, 0),
                  ([ok[:, :1].expand(8, 4)], 4, 3), ([torch.zeros(8, 3, 4, 5)[:, :2, :2, :2]], 4, 3),
-                 ([torch.zeros(20).as_strided((8, 4), (2, 1))], 4, 3)):
+                 ([torch.zeros(20).as_strided((8, 4), (2, 1))], 4, 3),
+                 ([torch.zeros(8, 4, requires_grad=True)], 4, 3)):
         with pytest.raises(ValueError):
             ops.PagePool(*args)
 
@@ -341,6 +361,16 @@ def test_bind_takes_over_a_table():
                 ([[-1, 0, 0]] * 3, [1, 0, 0])):
         with pytest.raises(ValueError):
             pool.bind(*bad)
+
+
+def test_books_of_another_pool_are_refused():
+    pools = [ops.PagePool([torch.zeros(8, 4)], 4, slots, width) for slots, width in ((4, 8), (8, 4))]
+    assert pools[0].meta.numel() != pools[1].meta.numel()
+    other = ops.PagePool([torch.zeros(8, 4)], 8, 4, 8)
+    other.extend([1], 9)
+    pools[0].meta.copy_(other.meta)
+    with pytest.raises(ops.PageError, match="8 tokens a page"):
+        pools[0].check()
 
 
 def test_clearing_leaves_pages_that_are_zero_already():
@@ -416,3 +446,33 @@ def test_a_checkpoint_carries_the_masks_and_the_pages(tmp_path):
     for a, b in zip(sequences(run[3], run[4]), sequences(again[3], again[4])):
         assert len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
     again[5].close()
+
+
+def test_the_training_example_draws_the_same_masks_after_a_resume(tmp_path):
+    """examples/train with --dropout: stopped after 5 steps and resumed, its last step draws what
+    an uninterrupted run's does and comes to the same loss."""
+    import os
+    import re
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+    def train(name, *steps):
+        os.makedirs(tmp_path / name, exist_ok=True)
+        for n in steps:
+            res = subprocess.run(
+                [sys.executable, os.path.join(root, "examples", "train", "train.py"), "--hidden",
+                 "32", "--layers", "2", "--batch", "2", "--seq", "8", "--dropout", "0.2", "--steps",
+                 str(n)], capture_output=True, text=True, timeout=300,
+                env=dict(os.environ, TPI_DATA_DIRECTORY=str(tmp_path / name), OMP_NUM_THREADS="1"))
+            assert res.returncode == 0, res.stdout + res.stderr
+        return re.findall(r"step 8 loss (\S+)", res.stdout), (tmp_path / name / ".ckpt-rank0")
+
+    from terraform_provider_iterative_amd.checkpoint.checkpointer import describe_checkpoint
+
+    (a, whole), (b, resumed) = train("whole", 8), train("resumed", 5, 8)
+    assert a and a == b
+    states = [describe_checkpoint(str(path))["metadata"]["training_state"]["stateful"]["masks"]
+              for path in (whole, resumed)]
+    assert states[0] == states[1] and states[0]["number"] == 18  # 2 a step, and the warm step's
