@@ -160,6 +160,33 @@ def _build(target: str, cmd: List[str], deps: Sequence[str], force: bool,
     return target
 
 
+def _build_objects(target: str, flags: Sequence[str], srcs: Sequence[str], link: Sequence[str],
+                   headers: Sequence[str], prefix: str, jobs: int, force: bool,
+                   verbose: bool) -> str:
+    """``target`` from objects compiled side by side (``flags`` + ``-c``), each with a stamp of its
+    own.  The target's stamp covers the sources, not the objects: a copy of the tree without them
+    (what a GPU box gets) is as fresh as the tree it was made from."""
+    objdir = os.path.join(LIB, "obj")
+    deps = [*srcs, *headers]
+    objs = [os.path.join(objdir, prefix + os.path.basename(src) + ".o") for src in srcs]
+    cmd = [c for part in link for c in (objs if part == "@OBJS@" else [part])]
+    key = [*flags, *cmd]
+    if not force and not _stale(target, key, deps):
+        _write_fast(target, deps)
+        return target
+    os.makedirs(objdir, exist_ok=True)
+    from concurrent.futures import ThreadPoolExecutor
+
+    with ThreadPoolExecutor(max(1, min(len(srcs), jobs))) as pool:
+        list(pool.map(lambda pair: _build(pair[1], [*flags, "-c", pair[0], "-o", "@OUT@"],
+                                          [pair[0], *headers], force, verbose), zip(srcs, objs)))
+    tmp = _atomic_output(target)
+    _run([tmp if c == "@OUT@" else c for c in cmd], verbose)
+    os.replace(tmp, target)
+    _stamp(target, key, deps)
+    return target
+
+
 def _define_version() -> str:
     return '-DTPI_VERSION_STRING="%s"' % version()
 
@@ -209,23 +236,11 @@ def build_hip(force: bool = False, verbose: bool = False) -> str:
     flags = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall",
              "-Wno-unused-function", "-munsafe-fp-atomics",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", _define_version()]
-    objdir = os.path.join(LIB, "obj")
-    os.makedirs(objdir, exist_ok=True)
-
-    def compile_one(src: str) -> str:
-        obj = os.path.join(objdir, os.path.basename(src) + ".o")
-        return _build(obj, [hipcc(), *flags, "-c", src, "-o", "@OUT@"], [src] + headers,
-                      force, verbose)
-
-    from concurrent.futures import ThreadPoolExecutor
-
-    jobs = max(1, min(len(srcs), int(os.environ.get("MAX_JOBS", "0") or os.cpu_count() or 4)))
-    with ThreadPoolExecutor(jobs) as pool:
-        objs = list(pool.map(compile_one, srcs))
-    cmd = [hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", *objs, "-L" + tl,
-           "-Wl,-rpath," + tl, "-L" + ROCM_LIB, "-Wl,-rpath," + ROCM_LIB, "-lrccl",
-           "-lrocprofiler-sdk-roctx", "-ldl", "-o", "@OUT@"]
-    return _build(HIP_SO, cmd, objs, force, verbose)
+    jobs = int(os.environ.get("MAX_JOBS", "0") or os.cpu_count() or 4)
+    link = [hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "@OBJS@", "-L" + tl,
+            "-Wl,-rpath," + tl, "-L" + ROCM_LIB, "-Wl,-rpath," + ROCM_LIB, "-lrccl",
+            "-lrocprofiler-sdk-roctx", "-ldl", "-o", "@OUT@"]
+    return _build_objects(HIP_SO, [hipcc(), *flags], srcs, link, headers, "", jobs, force, verbose)
 
 
 def build_supervisor(force: bool = False, verbose: bool = False) -> str:
@@ -278,20 +293,11 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     # torch's version file is a dependency: a different torch needs a rebuild
     headers = _sources("torchext/*.h", "common/*.h", "hip/tpi_hip.h") + [
         os.path.join(os.path.dirname(torch.__file__), "version.py")]
-    objdir = os.path.join(LIB, "obj")
-    os.makedirs(objdir, exist_ok=True)
-
-    def compile_one(src: str) -> str:
-        obj = os.path.join(objdir, "torchext_%s.o" % os.path.basename(src))
-        return _build(obj, [*flags, "-c", src, "-o", "@OUT@"], [src] + headers, force, verbose)
-
-    from concurrent.futures import ThreadPoolExecutor
-
-    with ThreadPoolExecutor(len(srcs)) as pool:  # torch's headers take a minute per source
-        objs = list(pool.map(compile_one, srcs))
-    cmd = [cxx, "-shared", "-fPIC", "-pthread", *objs, "-L" + tl, "-Wl,-rpath," + tl, "-lc10",
-           "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", "@OUT@"]
-    return _build(TORCH_EXT, cmd, objs, force, verbose)
+    link = [cxx, "-shared", "-fPIC", "-pthread", "@OBJS@", "-L" + tl, "-Wl,-rpath," + tl, "-lc10",
+            "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", "@OUT@"]
+    # torch's headers take a minute per source
+    return _build_objects(TORCH_EXT, flags, srcs, link, headers, "torchext_", len(srcs), force,
+                          verbose)
 
 
 def build_all(force: bool = False, verbose: bool = False, hip: bool = True) -> List[str]:
