@@ -1,13 +1,12 @@
 // Counter-based dropout as a differentiable torch operator (ops/masking.py): the host side of
 // every call -- output, view walked, launch -- and its autograd node, without Python in either
-// direction (a forward and a backward pass cost the host 120 us as Python functions).
+// direction: a forward and a backward pass cost the host 47 us (120 as Python functions; torch's own
+// dropout and addition 55, an addition alone 34).
 // Device tensors go to tpi_dropout (csrc/hip/dropout.hip); host tensors are computed here, to the
 // same bits.
-#include <c10/hip/HIPStream.h>
+#include <ATen/Parallel.h>
 #include <torch/extension.h>
 
-#include <algorithm>
-#include <thread>
 #include <vector>
 
 #include "../common/float16.h"
@@ -62,7 +61,7 @@ void dropout_range(const tpi_dropout_args& a, uint64_t seed, uint64_t draw, uint
   }
 }
 
-void dropout_host(const tpi_dropout_args& a, int threads) {
+void dropout_host(const tpi_dropout_args& a) {
   uint64_t seed = a.seed, draw = a.draw, total = 1;
   if (a.state) {
     seed = ((const uint64_t*)a.state)[0];
@@ -73,16 +72,9 @@ void dropout_host(const tpi_dropout_args& a, int threads) {
     ((uint64_t*)a.used)[1] = draw;
   }
   for (int d = 0; d < a.ndim; ++d) total *= (uint64_t)a.sizes[d];
-  const uint64_t least = 1 << 16;  // elements worth a thread
-  const int count = (int)std::max<uint64_t>(
-      1, std::min<uint64_t>((uint64_t)std::max(1, threads), total / least));
-  std::vector<std::thread> pool;
-  for (int t = 1; t < count; ++t)
-    pool.emplace_back([&, t] {
-      dropout_range(a, seed, draw, total * t / count, total * (t + 1) / count);
-    });
-  dropout_range(a, seed, draw, 0, total / count);
-  for (auto& t : pool) t.join();
+  at::parallel_for(0, (int64_t)total, 1 << 15, [&](int64_t lo, int64_t hi) {
+    dropout_range(a, seed, draw, (uint64_t)lo, (uint64_t)hi);
+  });
 }
 
 int type_of(at::ScalarType t) {
@@ -165,7 +157,7 @@ at::Tensor dropout_pass(const at::Tensor& x, const at::Tensor& residual, at::Sca
     a.ndim = merge(x.sizes(), strides, a);
   }
   if (x.is_cpu()) {
-    dropout_host(a, at::get_num_threads());
+    dropout_host(a);
     return out;
   }
   const c10::DeviceGuard guard(x.device());

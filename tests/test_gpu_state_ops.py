@@ -293,6 +293,24 @@ def test_many_slots_long_sequences_and_many_pages():
     _equal(host, dev)
 
 
+def test_more_pages_than_the_small_plan_takes():
+    pages = (1 << 20) + 77
+    base = torch.arange(16, dtype=torch.uint8).repeat(pages, 1) + \
+        (torch.arange(pages) % 251).to(torch.uint8)[:, None]
+    host, dev = [ops.PagePool([base.to(d)], 2, 4, pages) for d in ("cpu", "cuda")]
+    for pool in (host, dev):
+        pool.extend([0, 1, 2], [700001, 33, 1300001])
+        pool.free([0])
+        pool.fork([2], [0])
+        pool.extend([1, 3], [100000, 7])
+        pool.compact(clear=True)
+    _equal(host, dev)
+    for pool in (host, dev):
+        pool.free([1, 2])
+        pool.compact()
+    _equal(host, dev)
+
+
 @pytest.mark.parametrize("act,args,error", [
     ("extend", ([0, 1, 0], 1), "named twice"), ("extend", ([0, 9], 1), "slot is out of range"),
     ("extend", ([-1], 1), "slot is out of range"), ("extend", ([2], [-1]), "negative"),
