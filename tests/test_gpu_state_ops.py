@@ -78,7 +78,7 @@ def test_dropped_elements_are_zero_whatever_they_hold(bad):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("view", ["t", "slice", "expand", "permute", "step", "rows", "odd rows",
-                                  "offset", "one column"])
+                                  "offset", "one column", "heads", "blocks", "narrow blocks"])
 def test_dropout_of_views(view, dtype):
     base = _randn((12, 40, 48), dtype, 3)
 
@@ -87,7 +87,10 @@ def test_dropout_of_views(view, dtype):
                 "permute": lambda: b.permute(2, 0, 1), "expand": lambda: b[:, :1].expand(12, 5, 48),
                 "step": lambda: b[::2, :, ::3], "rows": lambda: b[:, :, 8:40],
                 "odd rows": lambda: b[:, :, 3:36], "offset": lambda: b.flatten()[1:],
-                "one column": lambda: b[:, :, 5]}[view]()
+                "one column": lambda: b[:, :, 5],
+                "heads": lambda: b.view(12, 40, 6, 8).transpose(1, 2),
+                "blocks": lambda: b.view(12, 8, 5, 48)[1:, ::3, 1:4, 8:40],
+                "narrow blocks": lambda: b.view(12, 8, 10, 24)[::2, 1:7, ::3, 4:7]}[view]()
 
     host, dev = pick(base), pick(base.cuda())
     r = _randn(host.shape, dtype, 4)
