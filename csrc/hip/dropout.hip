@@ -10,9 +10,9 @@
 //  k_dropout_rows     rows of unit stride, however they lie (a contiguous tensor is one row).  A
 //                     thread owns the 8 elements of a generator block: one 16-byte access (two for
 //                     fp32) each way.
-//  k_dropout_strided  views whose index does not run along memory (transposed, channels last): one
-//                     thread per element, which draws a block of its own.  16M bf16 elements 126 us,
-//                     as rows 13.5.
+//  k_dropout_tiles    views whose index runs across memory (transposed, channels last): a thread
+//                     owns the 8 x 8 elements of 8 generator blocks, 8 neighbours in memory each.
+//  k_dropout_strided  anything else: one thread per element, which draws a block of its own.
 #include <hip/hip_runtime.h>
 
 #include "../common/philox.h"
@@ -188,6 +188,66 @@ __global__ __launch_bounds__(kThreads) void k_dropout_rows(RowArgs a) {
       o[j] = apply<OUT, RES>((float)x[j], RES ? (float)r[j] : 0.0f, kept >> j & 1, a.scale);
 }
 
+struct TileArgs {
+  RowArgs row;                 // rows, per_row and outer: of tiles across `along`
+  int64_t along, across;       // sizes: of the index's dimension, of memory's
+  int64_t ax, ar, ao, ai;      // steps of the three operands along, of the index across
+};
+
+// Tiles of 8 elements along the index, which are one generator block, by 8 across it, which are
+// neighbours in memory.  Every block of the view is whole or cut at the dimension's end (the
+// host has checked: all steps of the index but this one are multiples of 8).  Lanes lie across,
+// so that their accesses join to whole lines.  16M bf16 elements, channels last: 16.2 us, 127 with
+// a thread and a block of the generator per element (contiguous: 13.3).
+template <int IN, int OUT, bool RES>
+__global__ __launch_bounds__(kThreads) void k_dropout_tiles(TileArgs t) {
+  typedef typename Elem<IN>::type TI;
+  typedef typename Elem<OUT>::type TO;
+  const RowArgs& a = t.row;
+  const Key key = read_key(a.state, a.used, a.seed, a.draw);
+  const int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t line = quotient(g, (int64_t)a.per_row, a.by_row, a.narrow);
+  if (line >= a.rows) return;
+  const int64_t b0 = (g - line * (int64_t)a.per_row) * 8;  // across
+  int64_t row = line;
+  uint64_t start = a.first;
+  int64_t sx = 0, sr = 0, so = 0, a0 = 0;
+  for (int k = a.outer - 1; k >= 0; --k) {  // the last one counts blocks along the index
+    const Outer& d = a.dim[k];
+    const int64_t q = k ? quotient(row, d.size, d.by, a.narrow) : 0, i = row - q * d.size;
+    sx += i * d.sx;
+    if (RES) sr += i * d.sr;
+    so += i * d.so;
+    start += (uint64_t)(i * d.si);
+    if (k == a.outer - 1) a0 = i * 8;
+    row = q;
+  }
+  const int na = (int)(t.along - a0 < 8 ? t.along - a0 : 8);
+  const int nb = (int)(t.across - b0 < 8 ? t.across - b0 : 8);
+  uint64_t kept = 0;  // bit 8 j + i: element i along, j across
+  for (int j = 0; j < nb; ++j)
+    kept |= (uint64_t)tpi_draw_block((start + (uint64_t)((b0 + j) * t.ai)) >> 3, key.draw, key.seed,
+                                     a.keep) << (8 * j);
+  const TI* x = (const TI*)a.x + sx + b0;
+  const TO* r = RES ? (const TO*)a.residual + sr + b0 : nullptr;
+  TO* o = (TO*)a.out + so + b0;
+  for (int i = 0; i < na; ++i, x += t.ax, r += RES ? t.ar : 0, o += t.ao, kept >>= 1) {
+    if (nb == 8) {
+      const Eight<TI> in = load8(x);
+      Eight<TO> out;
+      if (RES) out = load8(r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        out.e[j] = apply<OUT, RES>((float)in.e[j], RES ? (float)out.e[j] : 0.0f,
+                                   kept >> (8 * j) & 1, a.scale);
+      store8(o, out);
+    } else {
+      for (int j = 0; j < nb; ++j)
+        o[j] = apply<OUT, RES>((float)x[j], RES ? (float)r[j] : 0.0f, kept >> (8 * j) & 1, a.scale);
+    }
+  }
+}
+
 template <int IN, int OUT, bool RES>
 __global__ __launch_bounds__(kThreads) void k_dropout_strided(tpi_dropout_args a, uint64_t total) {
   typedef typename Elem<IN>::type TI;
@@ -222,20 +282,7 @@ Divider divider(uint64_t d) {
   return by;
 }
 
-template <int IN, int OUT, bool RES>
-int launch(const tpi_dropout_args& a, hipStream_t stream) {
-  uint64_t total = 1;
-  for (int d = 0; d < a.ndim; ++d) total *= (uint64_t)a.sizes[d];
-  const int last = a.ndim - 1;
-  const bool rows = a.sx[last] == 1 && a.so[last] == 1 && a.si[last] == 1 &&
-                    (!RES || a.sr[last] == 1);
-  if (!rows) {
-    const uint64_t want = (total + kThreads - 1) / kThreads;
-    const uint32_t grid = (uint32_t)(want < 65536 ? want : 65536);
-    k_dropout_strided<IN, OUT, RES><<<grid, kThreads, 0, stream>>>(a, total);
-    TPI_HIP(hipGetLastError());
-    return 0;
-  }
+RowArgs common(const tpi_dropout_args& a) {
   RowArgs k{};
   k.x = (const void*)a.x;
   k.residual = (const void*)a.residual;
@@ -247,28 +294,91 @@ int launch(const tpi_dropout_args& a, hipStream_t stream) {
   k.keep = tpi_keep_below(a.threshold);
   k.first = a.first;
   k.scale = a.scale;
-  k.cols = a.sizes[last];
   k.rows = 1;
-  k.outer = last;
-  uint64_t lead = a.first % 8;  // of a row's first element in its block; 7: of some row
   k.narrow = true;
+  return k;
+}
+
+void add_outer(RowArgs& k, int64_t size, int64_t sx, int64_t sr, int64_t so, int64_t si) {
+  k.dim[k.outer++] = Outer{size, sx, sr, so, si, divider((uint64_t)size)};
+  k.rows *= size;
+  k.narrow = k.narrow && size >> 31 == 0;
+}
+
+// Workgroups for per_row threads in each of the rows; 0: more than a launch has (2^32 threads, 34e9
+// elements of rows).
+uint32_t finish(RowArgs& k) {
+  k.by_row = divider(k.per_row);
+  const uint64_t threads = k.per_row * (uint64_t)k.rows;
+  // the last workgroup's threads behind the last block are divided, too
+  k.narrow = k.narrow && k.per_row >> 31 == 0 && (threads + kThreads) >> 31 == 0;
+  const uint64_t grid = (threads + kThreads - 1) / kThreads;
+  return grid * kThreads >> 32 ? 0 : (uint32_t)grid;
+}
+
+template <int IN, int OUT, bool RES>
+int launch_rows(const tpi_dropout_args& a, hipStream_t stream) {
+  const int last = a.ndim - 1;
+  RowArgs k = common(a);
+  k.cols = a.sizes[last];
+  uint64_t lead = a.first % 8;  // of a row's first element in its block; 7: of some row
   for (int d = 0; d < last; ++d) {
-    k.dim[d] = Outer{a.sizes[d], a.sx[d], RES ? a.sr[d] : 0, a.so[d], a.si[d],
-                     divider((uint64_t)a.sizes[d])};
-    k.rows *= a.sizes[d];
+    add_outer(k, a.sizes[d], a.sx[d], a.sr[d], a.so[d], a.si[d]);
     if (a.si[d] % 8) lead = 7;
-    k.narrow = k.narrow && a.sizes[d] >> 31 == 0;
   }
   k.per_row = ((uint64_t)k.cols + lead + 7) / 8;
-  k.by_row = divider(k.per_row);
-  const uint64_t blocks = k.per_row * (uint64_t)k.rows;
-  // the last workgroup's threads behind the last block are divided, too
-  k.narrow = k.narrow && k.per_row >> 31 == 0 && (blocks + kThreads) >> 31 == 0;
-  const uint64_t grid = (blocks + kThreads - 1) / kThreads;
-  // a launch has fewer than 2^32 threads: 34e9 elements
-  if (grid * kThreads >> 32) return tpi_fail("dropout: tensor too large");
+  const uint32_t grid = finish(k);
+  if (!grid) return tpi_fail("dropout: tensor too large");
   const auto kernel = last ? k_dropout_rows<IN, OUT, RES, false> : k_dropout_rows<IN, OUT, RES, true>;
-  kernel<<<(uint32_t)grid, kThreads, 0, stream>>>(k);
+  kernel<<<grid, kThreads, 0, stream>>>(k);
+  TPI_HIP(hipGetLastError());
+  return 0;
+}
+
+// `along`: the dimension that the index runs along, `across`: the one that memory does.
+template <int IN, int OUT, bool RES>
+int launch_tiles(const tpi_dropout_args& a, int along, int across, hipStream_t stream) {
+  TileArgs t{};
+  t.row = common(a);
+  t.along = a.sizes[along];
+  t.across = a.sizes[across];
+  t.ax = a.sx[along];
+  t.ar = a.sr[along];
+  t.ao = a.so[along];
+  t.ai = a.si[across];
+  for (int d = 0; d < a.ndim; ++d)
+    if (d != along && d != across)
+      add_outer(t.row, a.sizes[d], a.sx[d], a.sr[d], a.so[d], a.si[d]);
+  add_outer(t.row, (t.along + 7) / 8, 8 * t.ax, 8 * t.ar, 8 * t.ao, 8);
+  t.row.per_row = (uint64_t)(t.across + 7) / 8;
+  const uint32_t grid = finish(t.row);
+  if (!grid) return tpi_fail("dropout: tensor too large");
+  k_dropout_tiles<IN, OUT, RES><<<grid, kThreads, 0, stream>>>(t);
+  TPI_HIP(hipGetLastError());
+  return 0;
+}
+
+template <int IN, int OUT, bool RES>
+int launch(const tpi_dropout_args& a, hipStream_t stream) {
+  const auto unit = [&](int d) {
+    return a.sx[d] == 1 && a.so[d] == 1 && (!RES || a.sr[d] == 1);
+  };
+  const int last = a.ndim - 1;
+  if (unit(last) && a.si[last] == 1) return launch_rows<IN, OUT, RES>(a, stream);
+  int along = -1, across = -1;
+  bool whole = a.first % 8 == 0;  // every block begins with an element of the view
+  for (int d = 0; d < a.ndim; ++d) {
+    if (a.si[d] == 1) along = d;
+    else if (a.si[d] % 8) whole = false;
+    if (unit(d)) across = d;
+  }
+  if (whole && along >= 0 && across >= 0 && along != across)
+    return launch_tiles<IN, OUT, RES>(a, along, across, stream);
+  uint64_t total = 1;
+  for (int d = 0; d < a.ndim; ++d) total *= (uint64_t)a.sizes[d];
+  const uint64_t want = (total + kThreads - 1) / kThreads;
+  const uint32_t grid = (uint32_t)(want < 65536 ? want : 65536);
+  k_dropout_strided<IN, OUT, RES><<<grid, kThreads, 0, stream>>>(a, total);
   TPI_HIP(hipGetLastError());
   return 0;
 }

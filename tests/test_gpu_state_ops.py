@@ -78,7 +78,8 @@ def test_dropped_elements_are_zero_whatever_they_hold(bad):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("view", ["t", "slice", "expand", "permute", "step", "rows", "odd rows",
-                                  "offset", "one column", "heads", "blocks", "narrow blocks"])
+                                  "offset", "one column", "heads", "blocks", "narrow blocks",
+                                  "channels last", "turned", "turned part"])
 def test_dropout_of_views(view, dtype):
     base = _randn((12, 40, 48), dtype, 3)
 
@@ -90,6 +91,9 @@ def test_dropout_of_views(view, dtype):
                 "one column": lambda: b[:, :, 5],
                 "heads": lambda: b.view(12, 40, 6, 8).transpose(1, 2),
                 "blocks": lambda: b.view(12, 8, 5, 48)[1:, ::3, 1:4, 8:40],
+                "channels last": lambda: b.view(12, 40, 8, 6).permute(0, 3, 1, 2),
+                "turned": lambda: b.view(480, 48)[:, :47].t(),
+                "turned part": lambda: b.view(12, 40, 48).transpose(1, 2)[2:, 5:, :33],
                 "narrow blocks": lambda: b.view(12, 8, 10, 24)[::2, 1:7, ::3, 4:7]}[view]()
 
     host, dev = pick(base), pick(base.cuda())
@@ -121,6 +125,26 @@ def test_a_shard_has_the_wholes_mask(starts, shape):
     part = tuple(slice(a, a + n) for a, n in zip(starts, shape))
     for x in (whole.cuda()[part], whole[part].contiguous().cuda()):
         _same(ops.dropout(x, 0.4, (2, 3), shard=((4, 6, 2048), starts)), want[part])
+
+
+@pytest.mark.parametrize("rows,cols,starts", [((5, 48), (0, 33), (5, 0)), ((0, 41), (8, 40), (0, 8)),
+                                              ((3, 48), (0, 33), (3, 1))])
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_transposed_shard(rows, cols, starts, residual):
+    """Tiles cut at both ends; with an index that begins inside a block, element by element."""
+    whole = _randn((48, 40), torch.float16, 3)
+    x = whole.t().contiguous().cuda()[cols[0]:cols[1], rows[0]:rows[1]].t()
+    part = (slice(*rows), slice(*cols))
+    want = ops.dropout(whole[part].contiguous(), 0.4, (2, 3), shard=((50, 48), starts))
+    shard = ((50, 48), starts)
+    if not residual:
+        _same(ops.dropout(x, 0.4, (2, 3), shard=shard), want)
+        return
+    r = _randn(x.shape, torch.float16, 5)
+    want = ops.dropout(whole[part].contiguous(), 0.4, (2, 3), residual=r, shard=shard)
+    turned = r.t().contiguous().cuda().t()
+    _same(ops.dropout(x, 0.4, (2, 3), residual=turned, shard=shard), want)
+    _same(ops.dropout(x, 0.4, (2, 3), residual=r.cuda(), shard=shard), want)
 
 
 def test_more_elements_than_32_bits_count():
