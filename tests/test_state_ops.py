@@ -476,3 +476,134 @@ def test_the_training_example_draws_the_same_masks_after_a_resume(tmp_path):
     states = [describe_checkpoint(str(path))["metadata"]["training_state"]["stateful"]["masks"]
               for path in (whole, resumed)]
     assert states[0] == states[1] and states[0]["number"] == 18  # 2 a step, and the warm step's
+
+
+RANK_LOOP = r'''#!%(python)s
+import hashlib, os, signal, sys
+sys.path.insert(0, %(root)r)
+import torch
+from terraform_provider_iterative_amd import ops
+from terraform_provider_iterative_amd.checkpoint import TrainingState
+
+WHERE = os.environ.get("KILL_WHERE", "none")
+first = os.environ.get("TPI_RESTART_COUNT", "0") == "0"
+torch.set_num_threads(1)
+torch.manual_seed(0)
+masks = ops.MaskStream(5)
+model = torch.nn.Sequential(torch.nn.Linear(16, 32), ops.CounterDropout(0.3, masks),
+                            torch.nn.Linear(32, 16))
+opt = torch.optim.AdamW(model.parameters(), lr=1e-2)
+model(torch.zeros(1, 16)).sum().backward()
+opt.step()
+kv = torch.zeros(3, 40, 4, 16)
+pool = ops.PagePool(list(kv.unbind(0)), page_tokens=4, slots=6, width=10)
+state = TrainingState(model, opt, path=os.path.join(os.environ.get("TPI_DATA_DIRECTORY", "."),
+                                                   ".spill"), tile_bytes=4096,
+                      stateful={"masks": masks}, paged={"kv": pool})
+state.resume()
+start = state.step_value or 0
+print("start", start, "live", pool.status()["live"], flush=True)
+state.install()
+
+def kill(where, step):
+    if first and where == WHERE and step == 6:
+        os.kill(os.getpid(), signal.SIGTERM)
+
+def append(slots, rows):  # one token each
+    pool.extend(slots, 1)
+    for slot, row in zip(slots, rows):
+        at = int(pool.lengths[slot]) - 1
+        kv[:, int(pool.table[slot, at // 4]), at %% 4] = row
+
+for step in range(start, 12):
+    x = torch.randn(6, 16)
+    y = ops.dropout(model(x), 0.2, masks, residual=x)
+    kill("after-forward", step)
+    opt.zero_grad()
+    y.pow(2).mean().backward()
+    opt.step()
+    slots = [s for s in range(6) if (s + step) %% 3]
+    append(slots, y.detach()[slots])
+    kill("after-append", step)
+    if step %% 5 == 1:
+        pool.free([3, 5])
+        pool.fork([1, 2], [3, 5])
+    kill("after-fork", step)
+    state.step(step + 1)
+h = hashlib.sha256()
+for t in model.state_dict().values():
+    h.update(t.numpy().tobytes())
+for slot in range(6):
+    held = [int(p) for p in pool.table[slot] if p >= 0]
+    tokens = kv[:, held].reshape(3, -1, 16)[:, :int(pool.lengths[slot])]
+    h.update(tokens.contiguous().numpy().tobytes())
+print("final", h.hexdigest(), pool.lengths.tolist(), masks.state_dict(), flush=True)
+state.close()
+'''
+
+
+@pytest.fixture(scope="module")
+def uninterrupted(tmp_path_factory):
+    import os
+    import subprocess
+    import sys
+
+    d = tmp_path_factory.mktemp("rank")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = RANK_LOOP % {"python": sys.executable, "root": root}
+    (d / "loop.py").write_text(script)
+    env = dict(os.environ, TPI_DATA_DIRECTORY=str(d))
+    env.pop("TPI_EVENTS_FILE", None)
+    res = subprocess.run([sys.executable, str(d / "loop.py")], env=env, capture_output=True,
+                         text=True, timeout=300)
+    assert res.returncode == 0, res.stderr
+    return script, [line for line in res.stdout.splitlines() if line.startswith("final")][0]
+
+
+@pytest.mark.parametrize("where", ["after-forward", "after-append", "after-fork"])
+def test_a_preempted_rank_goes_on_with_its_masks_and_pages(tmp_path, uninterrupted, where):
+    """A rank that trains with dropout and keeps a paged cache is preempted inside a step: its
+    successor ends with the parameters and the cached tokens of an uninterrupted run."""
+    from terraform_provider_iterative_amd import backends
+    from terraform_provider_iterative_amd.models.cloud import Cloud, Credentials, NodeCredentials
+    from terraform_provider_iterative_amd.models.values import Environment, Task, Variables
+    from terraform_provider_iterative_amd.utils.identifier import new_deterministic_identifier
+
+    script, final = uninterrupted
+    cloud = Cloud(provider="local",
+                  credentials=Credentials(node=NodeCredentials(state_root=str(tmp_path / "st"))))
+    task = backends.new(cloud, new_deterministic_identifier("pages-" + where), Task(
+        environment=Environment(script=script, timeout=300, variables=Variables(
+            {"TPI_TASK": "true", "KILL_WHERE": where}))))
+    task.create()
+    status = task.wait(240)
+    logs = task.logs()
+    task.delete()
+    assert status["succeeded"] == 1 and len(logs) == 2, (status, logs)
+    assert "start 7 " in logs[1], logs
+    assert final in logs[1], (final, logs)
+
+
+def test_a_save_in_the_middle_of_a_step_leaves_the_pages(tmp_path, monkeypatch):
+    from terraform_provider_iterative_amd.checkpoint import preemption
+
+    kv = torch.ones(10, 4)
+    pool = ops.PagePool([kv], 4, 3, 4)
+    pool.extend([0, 1], [9, 3])
+    pool.free([0])
+    state = TrainingState(torch.nn.Linear(2, 2), path=str(tmp_path / "spill"), tile_bytes=4096,
+                          paged={"kv": pool})
+    before = pool.meta.clone()
+    monkeypatch.setattr(preemption, "_mid_step", True)
+    state.save({"step": 1})
+    assert torch.equal(pool.meta, before) and kv.all()
+    monkeypatch.setattr(preemption, "_mid_step", False)
+    state.save({"step": 2})
+    assert pool.table[1, 0] == 0 and not kv[1:].any()
+    state.close()
+
+
+def test_paged_caches_are_checked_when_the_state_is_built():
+    with pytest.raises(ValueError, match="paged 'kv' is on"):
+        pool = ops.PagePool([torch.zeros(4, 4)], 4, 1)
+        TrainingState(torch.nn.Linear(2, 2, device="meta"), paged={"kv": pool}, device="meta")
