@@ -54,7 +54,7 @@ struct RowArgs {
   Divider by_row;    // by per_row
   int32_t outer;     // dimensions of rows
   bool narrow;       // every quotient and divisor is below 2^31
-  Outer dim[TPI_MAX_DIMS - 1];
+  Outer dim[TPI_MAX_DIMS - 1];  // the innermost first
   tpi_keep keep;
   float scale;
 };
@@ -62,6 +62,33 @@ struct RowArgs {
 __device__ static inline int64_t quotient(int64_t n, int64_t d, Divider by, bool narrow) {
   if (!narrow) return n / d;
   return (__umulhi((uint32_t)n, by.mul) + (uint32_t)n) >> by.shift;
+}
+
+// Offsets of a row in the operands and in the index; returns its place in the innermost dimension.
+// That one is taken first, from a fixed place in the arguments: most views have no other.
+template <bool RES>
+__device__ static inline int64_t walk(const RowArgs& a, int64_t row, int64_t& sx, int64_t& sr,
+                                      int64_t& so, uint64_t& start) {
+  int64_t inner = row;
+  if (a.outer > 1) {
+    int64_t rest = quotient(row, a.dim[0].size, a.dim[0].by, a.narrow);
+    inner = row - rest * a.dim[0].size;
+    for (int k = 1; k < a.outer; ++k) {
+      const Outer& d = a.dim[k];
+      const int64_t q = k + 1 < a.outer ? quotient(rest, d.size, d.by, a.narrow) : 0;
+      const int64_t i = rest - q * d.size;
+      sx += i * d.sx;
+      if (RES) sr += i * d.sr;
+      so += i * d.so;
+      start += (uint64_t)(i * d.si);
+      rest = q;
+    }
+  }
+  sx += inner * a.dim[0].sx;
+  if (RES) sr += inner * a.dim[0].sr;
+  so += inner * a.dim[0].so;
+  start += (uint64_t)(inner * a.dim[0].si);
+  return inner;
 }
 
 // The draw's seed and number: from the call, or from device memory at the time the kernel runs.
@@ -148,15 +175,7 @@ __global__ __launch_bounds__(kThreads) void k_dropout_rows(RowArgs a) {
   const int64_t b = t - row * (int64_t)a.per_row;
   uint64_t start = a.first;  // index of the row's first element
   int64_t sx = 0, sr = 0, so = 0;
-  for (int k = ONE ? -1 : a.outer - 1; k >= 0; --k) {
-    const Outer& d = a.dim[k];
-    const int64_t q = k ? quotient(row, d.size, d.by, a.narrow) : 0, i = row - q * d.size;
-    sx += i * d.sx;
-    if (RES) sr += i * d.sr;
-    so += i * d.so;
-    start += (uint64_t)(i * d.si);
-    row = q;
-  }
+  if (!ONE) walk<RES>(a, row, sx, sr, so, start);
   const uint64_t block = (start >> 3) + (uint64_t)b;
   const int64_t c0 = b * 8 - (int64_t)(start & 7);  // column of the block's element 0
   if (c0 >= a.cols) return;
@@ -209,19 +228,9 @@ __global__ __launch_bounds__(kThreads) void k_dropout_tiles(TileArgs t) {
   const int64_t line = quotient(g, (int64_t)a.per_row, a.by_row, a.narrow);
   if (line >= a.rows) return;
   const int64_t b0 = (g - line * (int64_t)a.per_row) * 8;  // across
-  int64_t row = line;
   uint64_t start = a.first;
-  int64_t sx = 0, sr = 0, so = 0, a0 = 0;
-  for (int k = a.outer - 1; k >= 0; --k) {  // the last one counts blocks along the index
-    const Outer& d = a.dim[k];
-    const int64_t q = k ? quotient(row, d.size, d.by, a.narrow) : 0, i = row - q * d.size;
-    sx += i * d.sx;
-    if (RES) sr += i * d.sr;
-    so += i * d.so;
-    start += (uint64_t)(i * d.si);
-    if (k == a.outer - 1) a0 = i * 8;
-    row = q;
-  }
+  int64_t sx = 0, sr = 0, so = 0;
+  const int64_t a0 = 8 * walk<RES>(a, line, sx, sr, so, start);  // along
   const int na = (int)(t.along - a0 < 8 ? t.along - a0 : 8);
   const int nb = (int)(t.across - b0 < 8 ? t.across - b0 : 8);
   uint64_t kept = 0;  // bit 8 j + i: element i along, j across
@@ -322,7 +331,7 @@ int launch_rows(const tpi_dropout_args& a, hipStream_t stream) {
   RowArgs k = common(a);
   k.cols = a.sizes[last];
   uint64_t lead = a.first % 8;  // of a row's first element in its block; 7: of some row
-  for (int d = 0; d < last; ++d) {
+  for (int d = last - 1; d >= 0; --d) {
     add_outer(k, a.sizes[d], a.sx[d], a.sr[d], a.so[d], a.si[d]);
     if (a.si[d] % 8) lead = 7;
   }
@@ -346,10 +355,10 @@ int launch_tiles(const tpi_dropout_args& a, int along, int across, hipStream_t s
   t.ar = a.sr[along];
   t.ao = a.so[along];
   t.ai = a.si[across];
-  for (int d = 0; d < a.ndim; ++d)
+  add_outer(t.row, (t.along + 7) / 8, 8 * t.ax, 8 * t.ar, 8 * t.ao, 8);
+  for (int d = a.ndim - 1; d >= 0; --d)
     if (d != along && d != across)
       add_outer(t.row, a.sizes[d], a.sx[d], a.sr[d], a.so[d], a.si[d]);
-  add_outer(t.row, (t.along + 7) / 8, 8 * t.ax, 8 * t.ar, 8 * t.ao, 8);
   t.row.per_row = (uint64_t)(t.across + 7) / 8;
   const uint32_t grid = finish(t.row);
   if (!grid) return tpi_fail("dropout: tensor too large");
