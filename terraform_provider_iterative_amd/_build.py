@@ -165,7 +165,7 @@ def _build_objects(target: str, flags: Sequence[str], srcs: Sequence[str], link:
                    verbose: bool) -> str:
     """``target`` from objects compiled side by side (``flags`` + ``-c``), each with a stamp of its
     own.  The target's stamp covers the sources, not the objects: a copy of the tree without them
-    (what a GPU box gets) is as fresh as the tree it was made from."""
+    is as fresh as the tree it was made from."""
     objdir = os.path.join(LIB, "obj")
     deps = [*srcs, *headers]
     objs = [os.path.join(objdir, prefix + os.path.basename(src) + ".o") for src in srcs]
