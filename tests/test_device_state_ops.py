@@ -161,6 +161,43 @@ def test_more_elements_than_32_bits_count():
                            shard=((1 << 30, 1 << 30), ((1 << 30) - 3, 5))))
 
 
+@pytest.mark.parametrize("shape", [(0,), (3, 0, 5), ()])
+def test_dropout_of_nothing_and_of_one(shape):
+    x = torch.ones(shape, device="cuda", requires_grad=True)
+    masks = ops.MaskStream(3, device="cuda")
+    out = ops.dropout(x, 0.5, masks, residual=torch.zeros(shape, device="cuda"))
+    grad, = torch.autograd.grad(out, x, torch.ones(shape, device="cuda"))
+    assert out.shape == grad.shape == x.shape and torch.equal(out, grad)
+    _same(out, ops.dropout(torch.ones(shape), 0.5, (3, 0)))
+
+
+def test_two_graphs_of_one_pool_take_turns():
+    """Their launches share the pool's scratch: replayed one after the other they agree with the host."""
+    host, dev = _pools("odd", 64, 4, 6, 16)
+    for pool in (host, dev):
+        pool.extend([0, 1], [30, 21])
+    graphs = []
+    for src, dst in (([0, 1], [2, 3]), ([1, 0], [4, 5])):
+        s, d = (torch.tensor(v, device="cuda") for v in (src, dst))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dev.free(d)
+            dev.fork(s, d)
+            dev.extend(d, 3)
+        graphs.append((graph, src, dst, s, d))
+    for _ in range(3):
+        for graph, src, dst, _s, _d in graphs:
+            graph.replay()
+            host.free(dst)
+            host.fork(src, dst)
+            host.extend(dst, 3)
+            _equal(host, dev)
+        for pool in (host, dev):
+            pool.extend([0], 1)
+            pool.compact(clear=True)
+        _equal(host, dev)
+
+
 def test_dropout_on_a_side_stream():
     x = _randn((4096, 2048), torch.bfloat16, 1)
     want = ops.dropout(x, 0.3, (1, 2))
