@@ -112,37 +112,45 @@ class PagePool:
                           np.zeros(self.slots, np.int32))
 
     def _lay_out_tensors(self) -> None:
-        parts = []
+        parts, layouts = [], {}  # tensors mostly share one layout: cut it once
         for t in self.tensors:
-            elem = t.element_size()
-            strides = sorted((st, size) for st, size in zip(t.stride(), t.shape) if size > 1)
-            if any(st <= 0 or (i and st < strides[i - 1][0] * strides[i - 1][1])
-                   for i, (st, _) in enumerate(strides)):
-                raise ValueError("a pool's tensors must not overlap themselves")
-            dims = canonical_view(t.shape[1:], t.stride()[1:])
-            if dims[-1][1] != 1:  # elements with gaps between them: runs of one element
-                dims.append((1, 1))
-            if len(dims) > 2:
-                raise ValueError("a page's bytes must be contiguous runs with one stride between "
-                                 "them, not %s with strides %s" % (tuple(t.shape), t.stride()))
-            runs, run_stride = dims[0] if len(dims) == 2 else (1, 0)
-            parts.append(self._cut(t.data_ptr(), t.stride(0) * elem, runs, run_stride * elem,
-                                   dims[-1][0] * elem))
+            key = t.shape, t.stride(), t.element_size()
+            if key not in layouts:
+                layouts[key] = self._cut_page(t)
+            part = layouts[key].copy()
+            part["base"] += t.data_ptr()
+            parts.append(part)
         chunks = np.concatenate(parts)
         if len(chunks) >= 1 << 23:
             raise ValueError("the pages are too large")
         self._chunks = len(chunks)
         self._chunk = torch.from_numpy(chunks.view(np.uint8)).to(self.device)
 
+    def _cut_page(self, t: torch.Tensor) -> np.ndarray:
+        """Chunks of a page of ``t``, from its first byte."""
+        elem = t.element_size()
+        strides = sorted((st, size) for st, size in zip(t.stride(), t.shape) if size > 1)
+        if any(st <= 0 or (i and st < strides[i - 1][0] * strides[i - 1][1])
+               for i, (st, _) in enumerate(strides)):
+            raise ValueError("a pool's tensors must not overlap themselves")
+        dims = canonical_view(t.shape[1:], t.stride()[1:])
+        if dims[-1][1] != 1:  # elements with gaps between them: runs of one element
+            dims.append((1, 1))
+        if len(dims) > 2:
+            raise ValueError("a page's bytes must be contiguous runs with one stride between "
+                             "them, not %s with strides %s" % (tuple(t.shape), t.stride()))
+        runs, run_stride = dims[0] if len(dims) == 2 else (1, 0)
+        return self._cut(t.stride(0) * elem, runs, run_stride * elem, dims[-1][0] * elem)
+
     @staticmethod
-    def _cut(base: int, page_stride: int, runs: int, run_stride: int, run: int) -> np.ndarray:
-        """Chunks of one tensor's page: whole runs while several fit, pieces of one otherwise."""
+    def _cut(page_stride: int, runs: int, run_stride: int, run: int) -> np.ndarray:
+        """Chunks of a page: whole runs while several fit, pieces of one otherwise."""
         units = -(-run // 16)
         if units <= CHUNK_UNITS:
             step = CHUNK_UNITS // units
             rows = np.arange(0, runs, step)
             out = np.zeros(len(rows), _CHUNK)
-            out["base"] = base + rows * run_stride
+            out["base"] = rows * run_stride
             out["rows"] = np.minimum(step, runs - rows)
             out["row_bytes"], out["row_units"] = run, units
         else:
@@ -151,7 +159,7 @@ class PagePool:
             ends = np.minimum(starts + step, run)
             starts = np.minimum(starts, run - 16)  # not less than one unit
             out = np.zeros(runs * len(starts), _CHUNK)
-            out["base"] = (base + np.arange(runs)[:, None] * run_stride + starts).reshape(-1)
+            out["base"] = (np.arange(runs)[:, None] * run_stride + starts).reshape(-1)
             out["rows"] = 1
             out["row_bytes"] = np.tile(ends - starts, runs)
             out["row_units"] = (out["row_bytes"] + 15) // 16
