@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from reference_impls import PoolOracle, keep_mask
+from state_oracles import PoolOracle, keep_mask
 from terraform_provider_iterative_amd import ops
 from terraform_provider_iterative_amd.checkpoint import TrainingState
 from terraform_provider_iterative_amd.ops import masking

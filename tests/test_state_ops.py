@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from reference_impls import PoolOracle, dropout_oracle, keep_mask, philox4x32
+from state_oracles import PoolOracle, dropout_oracle, keep_mask, philox4x32
 from terraform_provider_iterative_amd import ops
 from terraform_provider_iterative_amd.checkpoint import TrainingState
 from terraform_provider_iterative_amd.ops import masking, paging
