@@ -447,7 +447,7 @@ class TrainingState:
             if name in self.stateful:
                 self.stateful[name].load_state_dict(from_jsonable(saved))
         for pool in self.paged.values():
-            pool.check()
+            pool.resumed()
 
     def resume(self, persist_path: Optional[str] = None) -> Optional[Dict]:
         """Restore device tensors (host region, else ``persist_path``) and host tensors;

@@ -319,14 +319,31 @@ class PagePool:
         return [self.pages, self.slots, self.width, self.page_tokens]
 
     # -- what the host may know ---------------------------------------------------------------
-    def check(self) -> None:
-        """Raise :class:`PageError` if an operation has been refused since the last check, or the
-        books are not this pool's (of a checkpoint of another one).  Waits for the device."""
+    def _read_header(self) -> List[int]:
         header = self._header.tolist()
         if header[_SHAPE:_SHAPE + 4] != self._shape():
             raise PageError("the books are those of a pool of %d pages, %d slots of %d pages and %d "
                             "tokens a page" % tuple(header[_SHAPE:_SHAPE + 4]))
-        code = header[_ERROR]
+        return header
+
+    def resumed(self) -> None:
+        """The books and the tensors have been restored from a checkpoint: raise
+        :class:`PageError` if they are another pool's.  A refusal that the saved run had not asked
+        for changed nothing, so it fails no resume: it stays for the next :meth:`check`, as it
+        would have without the preemption (on the host, whose operations raise their own refusals
+        at once, it is reported here as a warning)."""
+        code = self._read_header()[_ERROR]
+        if code and not self._on_device:
+            import warnings
+
+            self._header[_ERROR] = 0
+            warnings.warn("the checkpoint's pool had refused an operation: %s"
+                          % _ERRORS.get(code, "error %d" % code), stacklevel=2)
+
+    def check(self) -> None:
+        """Raise :class:`PageError` if an operation has been refused since the last check, or the
+        books are not this pool's (of a checkpoint of another one).  Waits for the device."""
+        code = self._read_header()[_ERROR]
         if code:
             self._header[_ERROR] = 0
             raise PageError(_ERRORS.get(code, "error %d" % code))

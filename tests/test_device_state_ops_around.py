@@ -1,0 +1,33 @@
+"""Operators on a rank's state on the MI355X (tests/test_device_state_ops.py) where they meet what
+surrounds them: checkpoints, streams, transformations of a program."""
+import pytest
+import torch
+
+from terraform_provider_iterative_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _require_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU visible")
+    ops.hip(required=True)
+
+
+def test_a_refusal_nobody_asked_for_is_still_there_after_a_resume():
+    """What a resume does with books that hold a refusal: it goes on, and the next check raises."""
+    pool = ops.PagePool([torch.zeros(8, 4, device="cuda")], 4, 3, 8)
+    pool.extend(torch.tensor([0], device="cuda"), 100)
+    saved = pool.meta.clone()
+    again = ops.PagePool([torch.zeros(8, 4, device="cuda")], 4, 3, 8)
+    again.meta.copy_(saved)
+    again.resumed()
+    with pytest.raises(ops.PageError, match="longer than a row"):
+        again.check()
+    again.extend(torch.tensor([0], device="cuda"), 10)
+    again.check()
+    other = ops.PagePool([torch.zeros(8, 4, device="cuda")], 2, 3, 8)
+    other.meta.copy_(saved)
+    with pytest.raises(ops.PageError, match="4 tokens a page"):
+        other.resumed()
