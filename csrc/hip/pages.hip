@@ -122,7 +122,8 @@ __device__ static inline void zero_chunk(const tpi_page_chunk& c, int64_t page) 
   }
 }
 
-// Workgroups (chunk, pair): nothing to look up or divide before the first load.
+// Workgroups (chunk, pair): nothing to look up or divide before the first load.  A free page that is
+// written is not known to be zero any more.
 __global__ __launch_bounds__(kBlock) void k_copy(tpi_pages p, const void* src, const void* dst,
                                                  int64_t n, bool wide) {
   for (int64_t i = blockIdx.y; i < n; i += gridDim.y) {
@@ -132,6 +133,9 @@ __global__ __launch_bounds__(kBlock) void k_copy(tpi_pages p, const void* src, c
       continue;
     }
     copy_chunk(p.chunk[blockIdx.x], s, d);
+    const uint32_t bit = 1u << (d & 31);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && s != d && (p.free_bits[d >> 5] & bit))
+      atomicOr(&p.stale_bits[d >> 5], bit);
   }
 }
 

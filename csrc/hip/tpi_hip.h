@@ -214,7 +214,8 @@ typedef struct tpi_pages {
 } tpi_pages;
 // `wide` bit 0: slot / page numbers are int64, else int32; bit 1: the same of `more`.
 // copy: page src[i] to page dst[i] in every tensor; no page may be a destination twice, nor a
-// destination and a source.  A pair with a number out of range is left out (EPAGE).
+// destination and a source.  A pair with a number out of range is left out (EPAGE).  A free
+// destination's stale bit is set.
 int tpi_pages_copy(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
                    uint64_t stream);
 // The next four change nothing when they refuse (the reason goes to the header); n <= slots.

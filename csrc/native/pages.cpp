@@ -61,8 +61,12 @@ struct Check {
 
 void pages_copy(const tpi_pages& p, const int64_t* src, const int64_t* dst, int64_t n) {
   for (int64_t i = 0; i < n; ++i) {
-    if (!page_ok(p, src[i]) || !page_ok(p, dst[i])) refuse(p, TPI_PAGES_EPAGE);
-    else if (src[i] != dst[i]) move_page(p, src[i], dst[i]);
+    if (!page_ok(p, src[i]) || !page_ok(p, dst[i])) {
+      refuse(p, TPI_PAGES_EPAGE);
+    } else if (src[i] != dst[i]) {
+      move_page(p, src[i], dst[i]);
+      if (get(p.free_bits, dst[i])) set(p.stale_bits, dst[i]);  // not known to be zero any more
+    }
   }
 }
 

@@ -252,10 +252,10 @@ class PagePool:
             raise ValueError("%s of %d slots, the pool has %d" % (name, count, self.slots))
 
     def copy(self, src: Numbers, dst: Numbers) -> None:
-        """Page ``src[i]`` to page ``dst[i]`` in every tensor; the books stay as they are.  No page
-        may be a destination twice, nor destination and source: of such a call on device numbers,
-        those destinations' content is undefined.  A pair with a number out of range is left
-        out."""
+        """Page ``src[i]`` to page ``dst[i]`` in every tensor; sequences and counts stay as they are (of
+        a free page that is written, :meth:`compact` knows to clear it).  No page may be a destination twice, nor
+        destination and source: of such a call on device numbers, those destinations' content is
+        undefined.  A pair with a number out of range is left out."""
         known = not self._on_device or not (isinstance(src, torch.Tensor) or
                                                   isinstance(dst, torch.Tensor))
         if known and set(map(int, src)) & set(map(int, dst)):

@@ -69,6 +69,8 @@ class PoolOracle:
     def copy(self, src, dst):
         for t in self.tensors:
             t[list(dst)] = t[list(src)].clone()
+        refs = self.refs  # a free page that is written is not known to be zero any more
+        self.stale |= {int(d) for s, d in zip(src, dst) if s != d and refs[d] == 0}
 
     def extend(self, slots, tokens):
         counts = [tokens] * len(slots) if isinstance(tokens, int) else tokens

@@ -31,3 +31,21 @@ def test_a_refusal_nobody_asked_for_is_still_there_after_a_resume():
     other.meta.copy_(saved)
     with pytest.raises(ops.PageError, match="4 tokens a page"):
         other.resumed()
+
+
+@pytest.mark.parametrize("as_tensor", [False, True])
+def test_clearing_reaches_free_pages_that_a_copy_wrote(as_tensor):
+    host, dev = [ops.PagePool([torch.ones(70, 9000, device=d)], 4, 2, 12) for d in ("cpu", "cuda")]
+    for pool in (host, dev):
+        pool.extend([0], 10)
+        pool.compact(clear=True)
+        for src, dst in (([0, 1], [69, 2]), ([69], [33])):
+            if as_tensor and pool is dev:
+                src, dst = (torch.tensor(v, device="cuda") for v in (src, dst))
+            pool.copy(src, dst)
+        assert pool.tensors[0][[33, 69]].all()
+    assert torch.equal(host.meta[8:], dev.meta[8:].cpu())
+    for pool in (host, dev):
+        pool.compact(clear=True)
+        assert pool.tensors[0][:3].all() and not pool.tensors[0][3:].any()
+    assert torch.equal(host.meta[8:], dev.meta[8:].cpu())

@@ -56,3 +56,16 @@ def test_the_books_of_another_pool_do_not_resume(tmp_path):
     with pytest.raises(ops.PageError, match="4 tokens a page"):
         state.resume()
     state.close()
+
+
+def test_clearing_reaches_free_pages_that_a_copy_wrote():
+    data = torch.ones(12, 4)
+    pool = ops.PagePool([data], 4, 2, 12)
+    pool.extend([0], 10)
+    pool.compact(clear=True)
+    pool.copy([0, 1], [9, 2])
+    assert data[9].all()
+    pool.copy([9], [7])
+    pool.compact(clear=True)
+    assert pool.refs.tolist() == [1] * 3 + [0] * 9
+    assert data[:3].all() and not data[3:].any()
