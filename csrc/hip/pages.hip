@@ -252,7 +252,9 @@ __global__ __launch_bounds__(kPlan) void k_reserve(tpi_pages p, const void* a, c
     if (need) atomicAdd(&s_total, (unsigned long long)need);
   }
   __syncthreads();
-  if (!s_error)
+  const bool sound = !s_error;
+  __syncthreads();  // every wave has read it before the first reason below is written
+  if (sound)
     for (int i = tid; i < n; i += kPlan)
       if (mark[FORK ? number(b, i, wide) : number(a, i, wide)] != i)
         atomicMax(&s_error, TPI_PAGES_EDUPLICATE);

@@ -49,3 +49,28 @@ def test_clearing_reaches_free_pages_that_a_copy_wrote(as_tensor):
         pool.compact(clear=True)
         assert pool.tensors[0][:3].all() and not pool.tensors[0][3:].any()
     assert torch.equal(host.meta[8:], dev.meta[8:].cpu())
+
+
+@pytest.mark.parametrize("act", ["extend", "fork"])
+def test_of_two_reasons_the_same_is_given_every_time(act):
+    """More entries than the small plan takes, a slot named twice and too few pages: as on every run,
+    and as for few entries, the reason with the higher number."""
+    pool = ops.PagePool([torch.zeros(700, 4, device="cuda")], 4, 3000, 700)
+    if act == "fork":
+        pool.extend([0], 3)  # a partial page: each fork takes one
+    slots = torch.arange(1, 1501, device="cuda")
+    slots[1499] = 5
+    source = torch.zeros_like(slots)
+    for _ in range(20):
+        if act == "extend":
+            pool.extend(slots, 1)
+        else:
+            pool.fork(source, slots)
+        assert pool.status()["error"] == "a slot is named twice"
+        with pytest.raises(ops.PageError, match="named twice"):
+            pool.check()
+    slots[1499] = 1500
+    pool.extend(slots, 1) if act == "extend" else pool.fork(source, slots)
+    with pytest.raises(ops.PageError, match="not enough free pages"):
+        pool.check()
+    assert pool.status()["live"] == (act == "fork")
