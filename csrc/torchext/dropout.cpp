@@ -115,19 +115,36 @@ int merge(at::IntArrayRef shape, const int64_t* const (&strides)[4], tpi_dropout
   return n;
 }
 
+// Where a tensor's first element is.  Not every tensor has memory for its elements: a wrapper
+// (DTensor, jagged, fake) has none of its own, a storage may have been shrunk or freed; their
+// address is null, or what lies behind it is not theirs.
+uint64_t address(const at::Tensor& t) {
+  TORCH_CHECK_TYPE(t.layout() == at::kStrided && !t.is_nested(),
+                   "dropout of a nested or sparse tensor is not supported");
+  uint64_t elements = (uint64_t)t.storage_offset() + 1;
+  for (int64_t d = 0; d < t.dim(); ++d) elements += (uint64_t)((t.size(d) - 1) * t.stride(d));
+  const void* p = t.const_data_ptr();
+  TORCH_CHECK_VALUE(p && elements * t.element_size() <= t.storage().nbytes(),
+                    "dropout needs tensors with memory of their own for all elements (of a "
+                    "distributed tensor, its local part)");
+  return (uint64_t)p;
+}
+
 at::Tensor dropout_pass(const at::Tensor& x, const at::Tensor& residual, at::ScalarType out_type,
-                 const Mask& mask, const at::Tensor& used) {
+                        const Mask& mask, const at::Tensor& used) {
+  TORCH_CHECK_TYPE(x.layout() == at::kStrided && !x.is_nested(),
+                   "dropout of a nested or sparse tensor is not supported");
   at::Tensor out = at::empty_like(residual.defined() ? residual : x, x.options().dtype(out_type));
   const int64_t n = x.numel();
   if (n == 0) return out;  // nor will the backward pass read `used`
   TORCH_CHECK(!x._is_zerotensor() && !(residual.defined() && residual._is_zerotensor()),
               "dropout of a tensor without storage");
   tpi_dropout_args a{};
-  a.x = (uint64_t)x.const_data_ptr();
-  a.residual = residual.defined() ? (uint64_t)residual.const_data_ptr() : 0;
-  a.out = (uint64_t)out.mutable_data_ptr();
-  a.state = mask.state.defined() ? (uint64_t)mask.state.const_data_ptr() : 0;
-  a.used = used.defined() ? (uint64_t)used.mutable_data_ptr() : 0;
+  a.x = address(x);
+  a.residual = residual.defined() ? address(residual) : 0;
+  a.out = address(out);
+  a.state = mask.state.defined() ? address(mask.state) : 0;
+  a.used = used.defined() ? address(used) : 0;
   a.seed = mask.seed;
   a.draw = mask.number;
   a.first = mask.first;

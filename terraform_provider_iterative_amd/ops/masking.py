@@ -165,7 +165,8 @@ def dropout(x: torch.Tensor, p: float, draw: Union[MaskStream, Draw, Tuple[int, 
     ``shard=(whole_shape, starts)`` says that ``x`` is the block of a tensor of ``whole_shape``
     that begins at ``starts``: it is masked as that block of the whole would be.
 
-    The result is enqueued on the current stream of ``x``'s device.
+    ``x`` and ``residual`` are strided tensors with memory of their own (of a DTensor, its local part
+    with ``shard=``).  The result is enqueued on the current stream of ``x``'s device.
     """
     if not isinstance(x, torch.Tensor) or not (x.is_cuda or x.is_cpu):
         raise TypeError("dropout needs a tensor on the GPU or the host")

@@ -69,3 +69,56 @@ def test_clearing_reaches_free_pages_that_a_copy_wrote():
     pool.compact(clear=True)
     assert pool.refs.tolist() == [1] * 3 + [0] * 9
     assert data[:3].all() and not data[3:].any()
+
+
+# -- tensors without memory of their own -----------------------------------------------------------
+
+@pytest.fixture
+def one_rank():
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    yield
+    dist.destroy_process_group()
+
+
+def _without_memory(kind):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import Shard, distribute_tensor
+
+    x = torch.ones(8, 4)
+    if kind == "distributed":
+        return distribute_tensor(x, init_device_mesh("cpu", (1,)), [Shard(0)])
+    if kind == "fake":
+        return FakeTensorMode().from_tensor(x)
+    if kind in ("jagged", "nested"):
+        layout = torch.jagged if kind == "jagged" else torch.strided
+        return torch.nested.nested_tensor([x[:3], x[3:]], layout=layout)
+    if kind in ("freed", "short"):
+        x.untyped_storage().resize_(0 if kind == "freed" else 64)
+        return x
+    return {"sparse": x.to_sparse, "csr": x.to_sparse_csr, "mkldnn": x.to_mkldnn}[kind]()
+
+
+@pytest.mark.parametrize("kind", ["distributed", "jagged", "nested", "freed", "short", "sparse",
+                                  "csr", "mkldnn"])
+def test_dropout_refuses_tensors_without_memory(kind, one_rank):
+    refused = (TypeError, ValueError, RuntimeError)
+    with pytest.raises(refused):
+        ops.dropout(_without_memory(kind), 0.5, (1, 2))
+    with pytest.raises(refused):
+        ops.dropout(torch.ones(8, 4), 0.5, (1, 2), residual=_without_memory(kind))
+    with pytest.raises(refused):
+        ops.dropout(_without_memory(kind).requires_grad_(True), 0.5, (1, 2))
+
+
+def test_dropout_refuses_a_state_without_memory():
+    state = torch.zeros(2, dtype=torch.int64)
+    state.untyped_storage().resize_(8)
+    with pytest.raises(ValueError, match="memory of their own"):
+        ops.dropout(torch.ones(8, 4), 0.5, ops.Draw(0, 0, state))
+
+
+def test_dropout_of_a_distributed_tensors_local_part(one_rank):
+    x = _without_memory("distributed")
+    want = ops.dropout(torch.ones(8, 4), 0.5, (1, 2))
+    assert torch.equal(ops.dropout(x.to_local(), 0.5, (1, 2), shard=((8, 4), (0, 0))), want)
