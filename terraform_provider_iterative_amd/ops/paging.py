@@ -48,6 +48,15 @@ def _pad4(words: int) -> int:
     return (words + 3) // 4 * 4
 
 
+def _has_memory(t: torch.Tensor) -> bool:
+    """Whether all elements lie in memory of the tensor's own: those of a wrapper (DTensor, fake, jagged)
+    or of a freed storage do not, and the kernels go by addresses."""
+    if t.layout is not torch.strided or t.is_nested or torch._is_zerotensor(t):
+        return False
+    span = t.storage_offset() + 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr() != 0 and span * t.element_size() <= t.untyped_storage().nbytes()
+
+
 class PagePool:
     """The pages of ``tensors`` and the ``slots`` sequences that hold them.
 
@@ -75,6 +84,8 @@ class PagePool:
         tensors = list(tensors)
         if not tensors or not all(isinstance(t, torch.Tensor) for t in tensors):
             raise ValueError("a pool needs at least one tensor")
+        if not all(map(_has_memory, tensors)):
+            raise ValueError("a pool's tensors must be strided ones with memory of their own")
         self.device = tensors[0].device
         if self.device.type not in ("cuda", "cpu"):
             raise ValueError("a pool's tensors must be on the GPU or the host")
@@ -218,6 +229,8 @@ class PagePool:
             if values.device != self.device:
                 raise ValueError("%s must be on %s" % (what, self.device))
             out = values.contiguous()
+            if out.numel() and not out.data_ptr():  # a wrapper's, or of a freed storage
+                raise ValueError("%s must have memory of their own" % what)
             if self._on_device:
                 return out
             out = out.to(torch.int64)

@@ -122,3 +122,27 @@ def test_dropout_of_a_distributed_tensors_local_part(one_rank):
     x = _without_memory("distributed")
     want = ops.dropout(torch.ones(8, 4), 0.5, (1, 2))
     assert torch.equal(ops.dropout(x.to_local(), 0.5, (1, 2), shard=((8, 4), (0, 0))), want)
+
+
+@pytest.mark.parametrize("kind", ["distributed", "fake", "jagged", "nested", "freed", "short", "sparse",
+                                  "csr", "mkldnn"])
+def test_a_pool_refuses_tensors_without_memory(kind, one_rank):
+    with pytest.raises((TypeError, ValueError, RuntimeError)):
+        ops.PagePool([torch.ones(8, 4), _without_memory(kind)], 4, 2)
+
+
+@pytest.mark.parametrize("kind", ["distributed", "fake", "freed"])
+def test_a_pool_refuses_numbers_without_memory(kind, one_rank):
+    pool = ops.PagePool([torch.ones(8, 4)], 4, 2)
+    slots = torch.zeros(1, dtype=torch.int64)
+    if kind == "freed":
+        slots.untyped_storage().resize_(0)
+    else:
+        slots = _without_memory(kind).to(torch.int64).flatten()[:1]
+    before = pool.meta.clone()
+    for call in (lambda: pool.extend(slots, 1), lambda: pool.extend([0], slots),
+                 lambda: pool.fork(slots, [1]), lambda: pool.free(slots),
+                 lambda: pool.copy(slots, [2]), lambda: pool.copy([2], slots)):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            call()
+    assert torch.equal(pool.meta, before)
