@@ -6,6 +6,7 @@
 // same bits.
 #include <ATen/Parallel.h>
 #include <torch/extension.h>
+#include <torch/library.h>
 
 #include <vector>
 
@@ -81,12 +82,19 @@ int type_of(at::ScalarType t) {
   return t == at::kFloat ? TPI_F32 : t == at::kHalf ? TPI_F16 : TPI_BF16;
 }
 
-// What names a mask and places a tensor in it.
+// What names a mask and places a tensor in it.  Numbers without a sign go through torch as the signed
+// ones of their bits.
 struct Mask : torch::CustomClassHolder {
-  uint64_t seed, number, first, threshold;
-  float scale;
+  int64_t threshold;
+  double scale;
+  int64_t seed, number;
+  std::optional<at::Tensor> state;  // {seed, number} on the device
+  int64_t first;
   std::vector<int64_t> strides;  // of the whole tensor's indexes; empty: x is the whole tensor
-  at::Tensor state;              // {seed, number} on the device, or undefined
+  Mask(int64_t threshold, double scale, int64_t seed, int64_t number,
+       const std::optional<at::Tensor>& state, int64_t first, at::IntArrayRef strides)
+      : threshold(threshold), scale(scale), seed(seed), number(number), state(state), first(first),
+        strides(strides.vec()) {}
 };
 
 // Views walked together, as dimensions that every operand has a stride for: those of size 1
@@ -130,35 +138,69 @@ uint64_t address(const at::Tensor& t) {
   return (uint64_t)p;
 }
 
-at::Tensor dropout_pass(const at::Tensor& x, const at::Tensor& residual, at::ScalarType out_type,
-                        const Mask& mask, const at::Tensor& used) {
+at::Tensor empty_out(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                     at::ScalarType dtype) {
   TORCH_CHECK_TYPE(x.layout() == at::kStrided && !x.is_nested(),
                    "dropout of a nested or sparse tensor is not supported");
-  at::Tensor out = at::empty_like(residual.defined() ? residual : x, x.options().dtype(out_type));
+  return at::empty_like(residual ? *residual : x, x.options().dtype(dtype));
+}
+
+#define TPI_DROPOUT_ARGS                                                                       \
+  const at::Tensor &x, const std::optional<at::Tensor>&residual, at::ScalarType dtype,         \
+      int64_t threshold, double scale, int64_t seed, int64_t number,                           \
+      const std::optional<at::Tensor>&state, int64_t first, at::IntArrayRef strides,           \
+      const std::optional<at::Tensor>&used
+
+bool two_words(const std::optional<at::Tensor>& t, const at::Tensor& x) {
+  return !t || (t->scalar_type() == at::kLong && t->numel() == 2 && t->is_contiguous() &&
+                t->device() == x.device());
+}
+
+bool type_ok(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+
+// What ops.dropout has checked; a traced program may be run on other tensors.
+void check_args(TPI_DROPOUT_ARGS) {
+  const at::ScalarType type = x.scalar_type();
+  TORCH_CHECK_TYPE(type_ok(type) && type_ok(dtype) &&
+                       (type == dtype || type == at::kFloat || dtype == at::kFloat) &&
+                       (!residual || residual->scalar_type() == dtype),
+                   "dropout: unsupported types");
+  TORCH_CHECK_VALUE(!residual || (residual->sizes() == x.sizes() && residual->device() == x.device()),
+                    "dropout: the residual must have x's shape and device");
+  TORCH_CHECK_VALUE(threshold >= 0 && threshold <= 1ll << 32 && number >= 0 && first >= 0,
+                    "dropout: a number is out of range");
+  TORCH_CHECK_VALUE(strides.empty() || (int64_t)strides.size() == x.dim(),
+                    "dropout: a stride of the whole tensor for each dimension");
+  TORCH_CHECK_VALUE(two_words(state, x) && two_words(used, x),
+                    "dropout: a draw's state must be two contiguous int64 on x's device");
+}
+
+// The operator itself, on the host and the device.
+at::Tensor dropout_kernel(TPI_DROPOUT_ARGS) {
+  check_args(x, residual, dtype, threshold, scale, seed, number, state, first, strides, used);
+  at::Tensor out = empty_out(x, residual, dtype);
   const int64_t n = x.numel();
   if (n == 0) return out;  // nor will the backward pass read `used`
-  TORCH_CHECK(!x._is_zerotensor() && !(residual.defined() && residual._is_zerotensor()),
-              "dropout of a tensor without storage");
   tpi_dropout_args a{};
   a.x = address(x);
-  a.residual = residual.defined() ? address(residual) : 0;
+  a.residual = residual ? address(*residual) : 0;
   a.out = address(out);
-  a.state = mask.state.defined() ? address(mask.state) : 0;
-  a.used = used.defined() ? address(used) : 0;
-  a.seed = mask.seed;
-  a.draw = mask.number;
-  a.first = mask.first;
-  a.threshold = mask.threshold;
-  a.scale = mask.scale;
+  a.state = state ? address(*state) : 0;
+  a.used = used ? address(*used) : 0;
+  a.seed = (uint64_t)seed;
+  a.draw = (uint64_t)number;
+  a.first = (uint64_t)first;
+  a.threshold = (uint64_t)threshold;
+  a.scale = (float)scale;
   a.in_type = type_of(x.scalar_type());
-  a.out_type = type_of(out_type);
-  if (mask.strides.empty() && x.is_contiguous() && out.is_contiguous() &&
-      (!residual.defined() || residual.is_contiguous())) {
+  a.out_type = type_of(dtype);
+  if (strides.empty() && x.is_contiguous() && out.is_contiguous() &&
+      (!residual || residual->is_contiguous())) {
     a.ndim = 1;
     a.sizes[0] = n;
     a.sx[0] = a.sr[0] = a.so[0] = a.si[0] = 1;
   } else {
-    std::vector<int64_t> index = mask.strides;
+    std::vector<int64_t> index = strides.vec();
     if (index.empty()) {
       index.resize(x.dim());
       int64_t step = 1;
@@ -167,11 +209,10 @@ at::Tensor dropout_pass(const at::Tensor& x, const at::Tensor& residual, at::Sca
         step *= x.size(d);
       }
     }
-    const int64_t* const strides[4] = {x.strides().data(),
-                                       residual.defined() ? residual.strides().data()
-                                                          : out.strides().data(),
-                                       out.strides().data(), index.data()};
-    a.ndim = merge(x.sizes(), strides, a);
+    const int64_t* const walked[4] = {x.strides().data(),
+                                      residual ? residual->strides().data() : out.strides().data(),
+                                      out.strides().data(), index.data()};
+    a.ndim = merge(x.sizes(), walked, a);
   }
   if (x.is_cpu()) {
     dropout_host(a);
@@ -182,30 +223,40 @@ at::Tensor dropout_pass(const at::Tensor& x, const at::Tensor& residual, at::Sca
   return out;
 }
 
-at::Tensor run(const at::Tensor& x, const at::Tensor& residual, at::ScalarType out_type,
-               const c10::intrusive_ptr<Mask>& mask);
+at::Tensor dropout_meta(TPI_DROPOUT_ARGS) { return empty_out(x, residual, dtype); }
+
+// The operator as torch knows it: whatever a program does to its operators (tracing, wrapped
+// tensors, differentiation) finds it there.
+at::Tensor call(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                at::ScalarType dtype, const Mask& mask, const std::optional<at::Tensor>& used) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("tpi::dropout", "")
+                             .typed<at::Tensor(TPI_DROPOUT_ARGS)>();
+  return op.call(x, residual, dtype, mask.threshold, mask.scale, mask.seed, mask.number, mask.state,
+                 mask.first, mask.strides, used);
+}
 
 // The gradient of a dropped element is 0, of a kept one the scale times the output's: the
 // operator itself, applied to the gradient (so it can be differentiated again).
 struct Dropout : torch::autograd::Function<Dropout> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
-                            const std::optional<at::Tensor>& added, int64_t out_type,
-                            const c10::intrusive_ptr<Mask>& mask) {
-    const at::Tensor residual = added.value_or(at::Tensor());
-    at::Tensor used;
+                            const std::optional<at::Tensor>& residual, at::ScalarType dtype,
+                            const c10::intrusive_ptr<Mask>& mask,
+                            std::optional<at::Tensor> used) {
     c10::intrusive_ptr<Mask> again = mask;
-    if (mask->state.defined() && x.requires_grad()) {
+    if (mask->state && x.requires_grad()) {
       // the state may have moved on by the time the backward pass runs
-      used = at::empty({2}, mask->state.options());
+      if (!used) used = at::empty({2}, mask->state->options());
       again = c10::make_intrusive<Mask>(*mask);
       again->state = used;
       again->number = 0;
     }
     ctx->saved_data["mask"] = c10::IValue::make_capsule(again);
     ctx->saved_data["type"] = (int64_t)x.scalar_type();
-    ctx->saved_data["residual"] = residual.defined() && residual.requires_grad();
+    ctx->saved_data["residual"] = residual && residual->requires_grad();
     ctx->saved_data["x"] = x.requires_grad();
-    return dropout_pass(x, residual, (at::ScalarType)out_type, *mask, used);
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return call(x, residual, dtype, *mask, used);
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -213,38 +264,44 @@ struct Dropout : torch::autograd::Function<Dropout> {
     const at::Tensor& grad = grads[0];
     at::Tensor dx, dr;
     if (grad.defined() && ctx->saved_data["x"].toBool())
-      dx = run(grad.resolve_neg(), at::Tensor(), (at::ScalarType)ctx->saved_data["type"].toInt(),
-               c10::static_intrusive_pointer_cast<Mask>(ctx->saved_data["mask"].toCapsule()));
+      dx = call(grad.resolve_neg(), std::nullopt,
+                (at::ScalarType)ctx->saved_data["type"].toInt(),
+                *c10::static_intrusive_pointer_cast<Mask>(ctx->saved_data["mask"].toCapsule()),
+                std::nullopt);
     if (ctx->saved_data["residual"].toBool()) dr = grad;
-    return {dx, dr, at::Tensor(), at::Tensor()};
+    return {dx, dr, at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
-at::Tensor run(const at::Tensor& x, const at::Tensor& residual, at::ScalarType out_type,
-               const c10::intrusive_ptr<Mask>& mask) {
-  if (at::GradMode::is_enabled() &&
-      (x.requires_grad() || (residual.defined() && residual.requires_grad())))
-    return Dropout::apply(x, residual.defined() ? std::optional<at::Tensor>(residual) : std::nullopt,
-                          (int64_t)out_type, mask);
-  return dropout_pass(x, residual, out_type, *mask, at::Tensor());
+at::Tensor dropout_autograd(TPI_DROPOUT_ARGS) {
+  const auto mask = c10::make_intrusive<Mask>(threshold, scale, seed, number, state, first, strides);
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
+    return Dropout::apply(x, residual, dtype, mask, used);
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return call(x, residual, dtype, *mask, used);
 }
 
 at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residual,
                    uint64_t threshold, double scale, uint64_t seed, uint64_t number,
                    const std::optional<at::Tensor>& state, uint64_t first,
-                   std::vector<int64_t> strides) {
-  auto mask = c10::make_intrusive<Mask>();
-  mask->seed = seed;
-  mask->number = number;
-  mask->first = first;
-  mask->threshold = threshold;
-  mask->scale = (float)scale;
-  mask->strides = std::move(strides);
-  if (state) mask->state = *state;
+                   const std::vector<int64_t>& strides) {
   // views that are negated lazily (the imaginary part of a conjugate) are written out
-  return run(x.resolve_neg(), residual ? residual->resolve_neg() : at::Tensor(),
-             residual ? residual->scalar_type() : x.scalar_type(), mask);
+  std::optional<at::Tensor> added;
+  if (residual) added = residual->resolve_neg();
+  return call(x.resolve_neg(), added, added ? added->scalar_type() : x.scalar_type(),
+              Mask((int64_t)threshold, scale, (int64_t)seed, (int64_t)number, state, (int64_t)first,
+                   strides),
+              std::nullopt);
 }
+
+TORCH_LIBRARY(tpi, m) {
+  m.def("dropout(Tensor x, Tensor? residual, ScalarType dtype, int threshold, float scale, int seed, "
+        "int number, Tensor? state, int first, int[] strides, Tensor(a!)? used=None) -> Tensor");
+}
+TORCH_LIBRARY_IMPL(tpi, CPU, m) { m.impl("dropout", &dropout_kernel); }
+TORCH_LIBRARY_IMPL(tpi, CUDA, m) { m.impl("dropout", &dropout_kernel); }
+TORCH_LIBRARY_IMPL(tpi, Meta, m) { m.impl("dropout", &dropout_meta); }
+TORCH_LIBRARY_IMPL(tpi, Autograd, m) { m.impl("dropout", &dropout_autograd); }
 
 }  // namespace
 

@@ -47,7 +47,8 @@ class MaskStream:
     With ``device`` the seed and number are held there and read when a kernel runs, so that a
     captured graph draws new masks at every replay: call :meth:`advance` once per step, inside
     the capture, after the step's last draw.  Without it a capture is refused, because every
-    replay would repeat the captured masks.
+    replay would repeat the captured masks; so are ``torch.jit.trace``, ``make_fx`` and
+    ``torch.export`` (they record a draw that is given as numbers, ``torch.ops.tpi.dropout``).
     """
 
     def __init__(self, seed: int = 0, number: int = 0, device=None):
@@ -66,6 +67,9 @@ class MaskStream:
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             raise ValueError("a captured graph would repeat this stream's masks at every replay: "
                              "give MaskStream a device")
+        if not torch.compiler.is_dynamo_compiling() and _is_traced():
+            raise ValueError("a traced program would repeat this stream's mask at every run: "
+                             "give dropout a draw of its own")
         self.number += 1
         return Draw(self.seed, self.number - 1)
 
@@ -91,6 +95,11 @@ class MaskStream:
             self._ahead = 0
         else:
             self.seed, self.number = seed, number
+
+
+def _is_traced() -> bool:
+    return torch._C._is_tracing() or \
+        torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
 
 
 def _signed(value: int) -> int:

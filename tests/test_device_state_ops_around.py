@@ -74,3 +74,32 @@ def test_of_two_reasons_the_same_is_given_every_time(act):
     with pytest.raises(ops.PageError, match="not enough free pages"):
         pool.check()
     assert pool.status()["live"] == (act == "fork")
+
+
+# -- transformations of a program ------------------------------------------------------------------
+
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+def test_a_graph_of_dropout_computes_dropout(mode):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def block(x):
+        x = x.detach().requires_grad_(True)
+        out = ops.dropout(x * 2, 0.4, (3, 7), residual=x.float())
+        return out.detach(), torch.autograd.grad(out.sum(), x)[0]
+
+    make = lambda d: torch.randn(6, 11, generator=torch.Generator().manual_seed(1)).bfloat16().to(d)
+    traced = make_fx(block, tracing_mode=mode)(torch.zeros(6, 11, dtype=torch.bfloat16, device="cuda"))
+    for got, want, host in zip(traced(make("cuda")), block(make("cuda")), block(make("cpu"))):
+        assert torch.equal(got, want) and torch.equal(got.cpu(), host)
+
+
+def test_dropout_refuses_tensors_without_memory():
+    """Refused on the host, before anything is launched."""
+    x = torch.ones(8, 4, device="cuda")
+    freed = torch.ones(8, 4, device="cuda")
+    freed.untyped_storage().resize_(0)
+    for call in (lambda: ops.dropout(freed, 0.5, (1, 2)),
+                 lambda: ops.dropout(x, 0.5, (1, 2), residual=freed),
+                 lambda: ops.PagePool([x, freed], 4, 2)):
+        with pytest.raises(ValueError, match="memory of their own"):
+            call()

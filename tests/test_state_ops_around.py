@@ -146,3 +146,100 @@ def test_a_pool_refuses_numbers_without_memory(kind, one_rank):
         with pytest.raises((TypeError, ValueError, RuntimeError)):
             call()
     assert torch.equal(pool.meta, before)
+
+
+# -- transformations of a program ------------------------------------------------------------------
+
+KEY = ((1 << 64) - 3, 7)  # a seed that has no sign
+
+
+def _block(x):
+    return ops.dropout(x * 2, 0.4, KEY, residual=x) + 1
+
+
+def _block_gradient(x):
+    x = x.detach().requires_grad_(True)
+    return torch.autograd.grad(_block(x).sum(), x)[0]
+
+
+def _live_state(x):
+    x = x.detach().requires_grad_(True)
+    y = ops.dropout(x, 0.4, ops.Draw(0, 2, STATE))
+    return torch.autograd.grad(y.sum(), x)[0]
+
+
+STATE = torch.tensor([5, 6])
+
+
+@pytest.mark.parametrize("mode", ["real", "fake", "symbolic"])
+@pytest.mark.parametrize("f", [_block, _block_gradient])
+def test_a_graph_of_dropout_computes_dropout(f, mode):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    traced = make_fx(f, tracing_mode=mode)(torch.randn(6, 11))
+    x = torch.randn(6, 11)
+    assert torch.equal(traced(x), f(x))
+
+
+def test_a_graph_of_a_draw_with_a_state():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    traced, x = make_fx(_live_state)(torch.randn(40)), torch.randn(40)
+    assert torch.equal(traced(x), ops.dropout(torch.ones(40), 0.4, (5, 8)))
+
+
+def test_a_traced_and_an_exported_program_compute_dropout():
+    traced = torch.jit.trace(_block, (torch.randn(6, 11),))
+    x = torch.randn(6, 11)
+    assert torch.equal(traced(x), _block(x))
+
+    class Net(torch.nn.Module):
+        def forward(self, x):
+            return _block(x)
+
+    assert torch.equal(torch.export.export(Net(), (x,)).module()(x), _block(x))
+
+
+@pytest.mark.parametrize("dtype,residual", [(torch.bfloat16, None), (torch.bfloat16, torch.float32),
+                                            (torch.float16, torch.float16)])
+def test_dropout_of_fake_tensors(dtype, residual):
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.ones(5, 7, dtype=dtype).t().requires_grad_(True)
+        r = None if residual is None else torch.ones(7, 5, dtype=residual)
+        out = ops.dropout(x, 0.5, (1, 2), residual=r)
+        grad, = torch.autograd.grad(out.sum(), x)
+    assert type(out) is type(grad) is FakeTensor
+    assert out.shape == grad.shape == (7, 5) and grad.dtype == dtype
+    assert out.dtype == (residual or dtype) and out.stride() == ((1, 7) if r is None else (5, 1))
+
+
+def test_a_stream_is_refused_in_a_trace():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    masks, x = ops.MaskStream(3), torch.ones(8)
+    for trace in (torch.jit.trace, lambda f, args: make_fx(f)(*args)):
+        with pytest.raises(ValueError, match="traced"):
+            trace(lambda v: ops.dropout(v, 0.5, masks), (x,))
+    assert masks.number == 0
+    compiled = torch.compile(lambda v: ops.dropout(v, 0.5, masks) * 2, backend="eager")
+    for number in range(3):
+        assert torch.equal(compiled(x), ops.dropout(x, 0.5, (3, number)) * 2)
+    assert masks.number == 3
+
+
+def test_the_operators_own_refusals():
+    """A traced program may be given other tensors than it was traced with."""
+    x = torch.ones(4, 4)
+    good = dict(x=x, residual=None, dtype=torch.float32, threshold=1 << 31, scale=2.0, seed=1, number=2,
+                state=None, first=0, strides=[])
+    assert torch.equal(torch.ops.tpi.dropout(**good), ops.dropout(x, 0.5, (1, 2)))
+    for bad in (dict(x=x.double()), dict(dtype=torch.float64), dict(dtype=torch.int16),
+                dict(x=x.half(), dtype=torch.bfloat16), dict(residual=x.half()),
+                dict(residual=torch.ones(4)), dict(threshold=-1), dict(threshold=(1 << 32) + 1),
+                dict(number=-1), dict(first=-1), dict(strides=[1]), dict(state=torch.zeros(2)),
+                dict(state=torch.zeros(3, dtype=torch.int64)),
+                dict(used=torch.zeros(1, dtype=torch.int64)), dict(x=x.to_sparse())):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            torch.ops.tpi.dropout(**{**good, **bad})
