@@ -273,8 +273,23 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
+// The tangent that forward mode carries with a tensor; undefined: none.
+at::Tensor tangent(const std::optional<at::Tensor>& t) {
+  return t && t->defined() ? t->_fw_grad(/*level=*/0) : at::Tensor();
+}
+
 at::Tensor dropout_autograd(TPI_DROPOUT_ARGS) {
   const auto mask = c10::make_intrusive<Mask>(threshold, scale, seed, number, state, first, strides);
+  const at::Tensor tx = tangent(x), tr = tangent(residual);
+  if ((tx.defined() || tr.defined()) && c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    // linear in both: the tangent is the operator, applied to x's, plus the residual's
+    std::optional<at::Tensor> added, turned;
+    if (residual) added = tr.defined() ? residual->_fw_primal(0) : *residual;
+    if (tr.defined()) turned = tr;
+    const at::Tensor out = call(tx.defined() ? x._fw_primal(0) : x, added, dtype, *mask, used);
+    return at::_make_dual(out, tx.defined() ? call(tx, turned, dtype, *mask, std::nullopt) : tr.clone(),
+                          0);
+  }
   if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
     return Dropout::apply(x, residual, dtype, mask, used);
   const at::AutoDispatchBelowADInplaceOrView below;

@@ -103,3 +103,18 @@ def test_dropout_refuses_tensors_without_memory():
                  lambda: ops.PagePool([x, freed], 4, 2)):
         with pytest.raises(ValueError, match="memory of their own"):
             call()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_forward_mode_carries_the_tangents(residual):
+    import torch.autograd.forward_ad as forward
+
+    x, tx, r, tr = (torch.randn(65, 33, generator=torch.Generator().manual_seed(i)).bfloat16()
+                    for i in range(4))
+    masks = ops.MaskStream(4, device="cuda")
+    with forward.dual_level():
+        out = ops.dropout(forward.make_dual(x.cuda(), tx.cuda()), 0.4, masks,
+                          residual=forward.make_dual(r.cuda(), tr.cuda()) if residual else None)
+        primal, tangent = forward.unpack_dual(out)
+    assert torch.equal(primal.cpu(), ops.dropout(x, 0.4, (4, 0), residual=r if residual else None))
+    assert torch.equal(tangent.cpu(), ops.dropout(tx, 0.4, (4, 0), residual=tr if residual else None))

@@ -243,3 +243,49 @@ def test_the_operators_own_refusals():
                 dict(used=torch.zeros(1, dtype=torch.int64)), dict(x=x.to_sparse())):
         with pytest.raises((TypeError, ValueError, RuntimeError)):
             torch.ops.tpi.dropout(**{**good, **bad})
+
+
+@pytest.mark.parametrize("dtype,kind", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                        (torch.float16, torch.float16)])
+@pytest.mark.parametrize("which", ["x", "residual", "both"])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_carries_the_tangents(dtype, kind, which, requires_grad):
+    """The operator is linear: its tangent is itself, of x's tangent, plus the residual's."""
+    import torch.autograd.forward_ad as forward
+
+    g = torch.Generator().manual_seed(5)
+    x, tx = (torch.randn(9, 21, generator=g).to(dtype) for _ in range(2))
+    r, tr = (torch.randn(9, 21, generator=g).to(kind) for _ in range(2))
+    with forward.dual_level():
+        a = x.clone().requires_grad_(requires_grad)
+        b = r.clone().requires_grad_(requires_grad)
+        out = ops.dropout(a if which == "residual" else forward.make_dual(a, tx), 0.4, KEY,
+                          residual=b if which == "x" else forward.make_dual(b, tr))
+        primal, tangent = forward.unpack_dual(out)
+        assert torch.equal(primal, ops.dropout(x, 0.4, KEY, residual=r))
+        want = {"x": lambda: ops.dropout(tx, 0.4, KEY, residual=torch.zeros_like(r)),
+                "residual": lambda: tr, "both": lambda: ops.dropout(tx, 0.4, KEY, residual=tr)}
+        assert tangent.dtype == kind and torch.equal(tangent, want[which]())
+        if requires_grad:
+            grads = torch.autograd.grad(primal.sum(), (a, b))
+            assert torch.equal(grads[0], ops.dropout(torch.ones_like(x), 0.4, KEY))
+            assert torch.equal(grads[1], torch.ones_like(r))
+    alone = torch.func.jvp(lambda v: ops.dropout(v, 0.4, KEY), (x,), (tx,))[1]
+    assert torch.equal(alone, ops.dropout(tx, 0.4, KEY))
+
+
+def test_forward_mode_of_a_state_and_over_the_reverse():
+    import torch.autograd.forward_ad as forward
+
+    x, tx, w = (torch.randn(30, generator=torch.Generator().manual_seed(i)) for i in range(3))
+    with forward.dual_level():
+        v = forward.make_dual(x.clone().requires_grad_(True), tx)
+        out = ops.dropout(v, 0.4, ops.Draw(0, 2, STATE))
+        assert torch.equal(forward.unpack_dual(out).tangent, ops.dropout(tx, 0.4, (5, 8)))
+        # d/dt of the gradient of sum(w out^2): the operator, applied to 2 w times the tangent
+        gradient, = torch.autograd.grad((w * out ** 2).sum(), v, create_graph=True)
+        want = ops.dropout(2 * w * ops.dropout(tx, 0.4, (5, 8)), 0.4, (5, 8))
+        assert torch.allclose(forward.unpack_dual(gradient).tangent, want)
+    torch.autograd.gradcheck(lambda a, b: ops.dropout(a, 0.4, KEY, residual=b).double(),
+                             (torch.ones(11, requires_grad=True), torch.ones(11, requires_grad=True)),
+                             eps=0.25, atol=1e-5, check_forward_ad=True)
