@@ -236,6 +236,11 @@ at::Tensor call(const at::Tensor& x, const std::optional<at::Tensor>& residual,
                  mask.first, mask.strides, used);
 }
 
+// A gradient has whatever layout the rest of the graph gave it.  One of more dimensions than a launch
+// walks may not merge into those where the forward pass's operands did; laid out in order, it
+// does wherever they did.
+at::Tensor walkable(const at::Tensor& t) { return t.dim() > TPI_MAX_DIMS ? t.contiguous() : t; }
+
 // The gradient of a dropped element is 0, of a kept one the scale times the output's: the
 // operator itself, applied to the gradient (so it can be differentiated again).
 struct Dropout : torch::autograd::Function<Dropout> {
@@ -264,7 +269,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     const at::Tensor& grad = grads[0];
     at::Tensor dx, dr;
     if (grad.defined() && ctx->saved_data["x"].toBool())
-      dx = call(grad.resolve_neg(), std::nullopt,
+      dx = call(walkable(grad.resolve_neg()), std::nullopt,
                 (at::ScalarType)ctx->saved_data["type"].toInt(),
                 *c10::static_intrusive_pointer_cast<Mask>(ctx->saved_data["mask"].toCapsule()),
                 std::nullopt);

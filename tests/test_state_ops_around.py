@@ -289,3 +289,40 @@ def test_forward_mode_of_a_state_and_over_the_reverse():
     torch.autograd.gradcheck(lambda a, b: ops.dropout(a, 0.4, KEY, residual=b).double(),
                              (torch.ones(11, requires_grad=True), torch.ones(11, requires_grad=True)),
                              eps=0.25, atol=1e-5, check_forward_ad=True)
+
+
+# -- gradients and tangents of layouts that the caller did not choose ------------------------------
+
+def _turned(t):
+    """The same values, no two dimensions of which can be walked as one."""
+    order = list(range(t.dim()))[::-1]
+    return t.permute(order).contiguous().permute(order)
+
+
+@pytest.mark.parametrize("shard", [None, ((2,) * 6 + (5,), (0,) * 6 + (1,))])
+def test_a_gradient_of_many_dimensions_in_any_layout(shard):
+    x = torch.randn([2] * 6 + [3], requires_grad=True)
+    out = ops.dropout(x, 0.4, KEY, shard=shard)
+    grad = torch.randn(x.shape)
+    assert _turned(grad).stride() != grad.stride()
+    want = ops.dropout(grad, 0.4, KEY, shard=shard)
+    dx, = torch.autograd.grad(out, x, _turned(grad).requires_grad_(True), create_graph=True)
+    assert torch.equal(dx, want)
+
+
+def test_a_tangent_of_many_dimensions_in_any_layout():
+    x, t, r = (torch.randn([2] * 7) for _ in range(3))
+    got = torch.func.jvp(lambda a, b: ops.dropout(a, 0.4, KEY, residual=b), (x, r),
+                         (_turned(t), _turned(t) * 2))[1]
+    assert torch.equal(got, ops.dropout(t, 0.4, KEY, residual=t * 2))
+
+
+@pytest.mark.parametrize("dtype,kind", [(torch.float32, None), (torch.bfloat16, torch.float32)])
+def test_a_gradient_without_storage_is_a_zero_one(dtype, kind):
+    x = torch.randn(6, 5).to(dtype).requires_grad_(True)
+    r = None if kind is None else torch.randn(6, 5).to(kind).requires_grad_(True)
+    out = ops.dropout(x, 0.4, KEY, residual=r)
+    zero = torch._efficientzerotensor((6, 5), dtype=out.dtype)
+    grads = torch.autograd.grad(out, (x,) if r is None else (x, r), zero)
+    for grad, of in zip(grads, (x, r)):
+        assert grad.dtype == of.dtype and grad.shape == of.shape and not grad.any()
