@@ -402,6 +402,16 @@ int launch(const tpi_dropout_args& a, hipStream_t s) {
 
 }  // namespace
 
+extern "C" int tpi_capture_id(uint64_t stream, uint64_t* id) {
+  *id = 0;
+  if (!stream) return 0;  // the default stream is never captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long number = 0;
+  TPI_HIP(hipStreamGetCaptureInfo((hipStream_t)stream, &status, &number));
+  if (status != hipStreamCaptureStatusNone) *id = number + 1;  // whatever the first one's is
+  return 0;
+}
+
 extern "C" int tpi_dropout(const tpi_dropout_args* args, uint64_t stream) {
   const tpi_dropout_args& a = *args;
   if (a.ndim < 1 || a.ndim > TPI_MAX_DIMS) return tpi_fail("dropout: bad number of dimensions");

@@ -57,7 +57,7 @@ typedef struct tpi_stats {
 } tpi_stats;
 
 // Bumped whenever a signature below changes (ops/_loader.py checks it).
-#define TPI_ABI_VERSION 8
+#define TPI_ABI_VERSION 9
 
 // Library / device
 const char* tpi_last_error(void);
@@ -168,6 +168,8 @@ typedef struct tpi_dropout_args {
   int32_t ndim;
 } tpi_dropout_args;
 int tpi_dropout(const tpi_dropout_args* args, uint64_t stream);
+// The number of the capture that a stream is part of; 0: it is not being captured.
+int tpi_capture_id(uint64_t stream, uint64_t* id);
 
 // ---- Pages of a paged cache (ops/paging.py) ----------------------------------------------------
 // What one workgroup moves of a page: `rows` runs of `row_bytes` bytes in a tensor whose first

@@ -50,12 +50,18 @@ PYBIND11_MODULE(_tpi_torch, m) {
     }
   });
   m.def("use_hip", [](const std::vector<uintptr_t>& at) {
-    if (at.size() != 7) throw std::invalid_argument("use_hip: addresses of 7 entry points");
+    if (at.size() != 8) throw std::invalid_argument("use_hip: addresses of 8 entry points");
     tpi::g_hip = {(decltype(&tpi_last_error))at[0],  (decltype(&tpi_dropout))at[1],
                   (decltype(&tpi_pages_copy))at[2],  (decltype(&tpi_pages_fork))at[3],
                   (decltype(&tpi_pages_extend))at[4], (decltype(&tpi_pages_free))at[5],
-                  (decltype(&tpi_pages_compact))at[6]};
+                  (decltype(&tpi_pages_compact))at[6], (decltype(&tpi_capture_id))at[7]};
   });
+  m.def("stream_and_capture", [](int device) {
+    const uint64_t stream = tpi::current_stream(device);
+    uint64_t capture = 0;
+    tpi::hip_check(tpi::hip_api().capture_id(stream, &capture), "capture_id");
+    return std::make_pair(stream, capture);
+  }, "current stream of a device, and the number of the capture that it is part of (0: none)");
   tpi::bind_dropout(m);
   tpi::bind_pages(m);
   m.def("empty", &empty_nogil, "at::empty(shape, like.options()) with the GIL released",

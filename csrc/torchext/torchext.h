@@ -20,6 +20,7 @@ struct HipApi {
   decltype(&tpi_pages_extend) pages_extend;
   decltype(&tpi_pages_free) pages_free;
   decltype(&tpi_pages_compact) pages_compact;
+  decltype(&tpi_capture_id) capture_id;
 };
 const HipApi& hip_api();  // throws when the library has not been handed over
 

@@ -14,7 +14,7 @@ from typing import Optional
 
 from .. import _build
 
-ABI_VERSION = 8  # TPI_ABI_VERSION of csrc/hip/tpi_hip.h
+ABI_VERSION = 9  # TPI_ABI_VERSION of csrc/hip/tpi_hip.h
 
 _lock = threading.Lock()
 _native = None
@@ -81,7 +81,7 @@ def torch_hip():
         lib, ext = hip(), torch_ext()
         ext.use_hip([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "tpi_last_error", "tpi_dropout", "tpi_pages_copy", "tpi_pages_fork",
-            "tpi_pages_extend", "tpi_pages_free", "tpi_pages_compact")])
+            "tpi_pages_extend", "tpi_pages_free", "tpi_pages_compact", "tpi_capture_id")])
         _torch_hip = ext
     return _torch_hip
 
@@ -141,6 +141,7 @@ class HipLib:
             "tpi_pack_device": (i32, [vp, vp, i32, u64, vp, u64, vp, u64]),
             "tpi_unpack_device": (i32, [vp, vp, i32, u64, vp, u64, vp, vp, u64]),
             "tpi_dropout": (i32, [c.c_char_p, u64]),
+            "tpi_capture_id": (i32, [u64, vp]),
             "tpi_pages_copy": (i32, [c.c_char_p, vp, vp, i64, i32, u64]),
             "tpi_pages_fork": (i32, [c.c_char_p, vp, vp, i64, i32, u64]),
             "tpi_pages_extend": (i32, [c.c_char_p, vp, i64, i32, vp, i64, u64]),

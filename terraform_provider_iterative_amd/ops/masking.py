@@ -27,7 +27,8 @@ _WHOLE = 1 << 32
 
 class Draw(NamedTuple):
     """What names one mask: ``(seed, number)``, or with ``state`` (an int64 tensor ``[seed,
-    number]`` on the operand's device) ``state``'s seed and ``number`` past ``state``'s."""
+    number]`` on the operand's device) ``state``'s seed and ``number`` past ``state``'s, which are
+    read when a kernel runs (a :class:`MaskStream` gives its draws a state that stays as it is)."""
     seed: int
     number: int
     state: Optional[torch.Tensor] = None
@@ -46,7 +47,8 @@ class MaskStream:
 
     With ``device`` the seed and number are held there and read when a kernel runs, so that a
     captured graph draws new masks at every replay: call :meth:`advance` once per step, inside
-    the capture, after the step's last draw.  Without it a capture is refused, because every
+    the capture, after the step's last draw.  A draw keeps its mask, also once the stream has
+    advanced (a block that the backward pass computes again).  Without it a capture is refused, because every
     replay would repeat the captured masks; so are ``torch.jit.trace``, ``make_fx`` and
     ``torch.export`` (they record a draw that is given as numbers, ``torch.ops.tpi.dropout``).
     """
@@ -59,11 +61,23 @@ class MaskStream:
             self.state = torch.tensor([_signed(self.seed), self.number], dtype=torch.int64,
                                       device=device)
             self._ahead = 0
+            self._copies: dict = {}
+
+    def _copy(self) -> torch.Tensor:
+        """What this step's draws refer to: a copy of the state, which advancing does not change.  One
+        for each stream and each captured graph that draws, ordered before what it draws."""
+        where = torch_hip().stream_and_capture(self.state.device.index) if self.state.is_cuda else 0
+        copy = None if _is_traced() else self._copies.get(where)
+        if copy is None:
+            copy = self.state + 0  # a kernel
+            if type(copy) is torch.Tensor and not _is_traced():  # not a recording's
+                self._copies[where] = copy
+        return copy
 
     def next(self) -> Draw:
         if self.state is not None:
             self._ahead += 1
-            return Draw(0, self._ahead - 1, self.state)
+            return Draw(0, self._ahead - 1, self._copy())
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             raise ValueError("a captured graph would repeat this stream's masks at every replay: "
                              "give MaskStream a device")
@@ -78,7 +92,7 @@ class MaskStream:
         if self.state is None:
             raise ValueError("advance() is for a MaskStream with a device")
         self.state[1:].add_(self._ahead)
-        self._ahead = 0
+        self._ahead, self._copies = 0, {}
 
     def state_dict(self) -> dict:
         seed, number = self.seed, self.number
@@ -92,7 +106,7 @@ class MaskStream:
         _check_key(seed, number)
         if self.state is not None:
             self.state.copy_(torch.tensor([_signed(seed), number], dtype=torch.int64))
-            self._ahead = 0
+            self._ahead, self._copies = 0, {}
         else:
             self.seed, self.number = seed, number
 

@@ -118,3 +118,74 @@ def test_forward_mode_carries_the_tangents(residual):
         primal, tangent = forward.unpack_dual(out)
     assert torch.equal(primal.cpu(), ops.dropout(x, 0.4, (4, 0), residual=r if residual else None))
     assert torch.equal(tangent.cpu(), ops.dropout(tx, 0.4, (4, 0), residual=tr if residual else None))
+
+
+# -- blocks that are computed twice ----------------------------------------------------------------
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_block_computed_twice_after_the_stream_has_advanced(captured):
+    """Activation checkpointing with the draw taken outside; in a graph every replay draws anew."""
+    from torch.utils.checkpoint import checkpoint
+
+    masks = ops.MaskStream(21, device="cuda")
+    w = torch.randn(64, 64, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_(True)
+    x = torch.randn(32, 64, generator=torch.Generator().manual_seed(2)).cuda().requires_grad_(True)
+
+    def block(v, draw):
+        return (ops.dropout(v * w[0], 0.5, draw) * w[1]).pow(2)
+
+    def step(one, two):
+        y = checkpoint(block, checkpoint(block, x, one, use_reentrant=False), two, use_reentrant=False)
+        if one is not None and isinstance(one, ops.Draw) and one.state is not None:
+            masks.advance()
+        return torch.autograd.grad(y.sum(), (x, w))
+
+    def check(got, number):
+        want = step((21, number), (21, number + 1))
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+    if not captured:
+        for number in range(0, 6, 2):
+            check(step(masks.next(), masks.next()), number)
+        return
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(masks.next(), masks.next())
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(masks.next(), masks.next())
+    for replay in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        check(got, 2 + 2 * replay)
+        assert masks.state_dict()["number"] == 4 + 2 * replay
+
+
+def test_draws_of_a_step_in_several_graphs_and_streams():
+    """A step whose draws are captured in two graphs, with eager ones of the same step before and
+    between: none of them refers to what another capture, or an eager draw, has copied."""
+    masks, x = ops.MaskStream(5, device="cuda"), torch.ones(512, device="cuda")
+    ops.dropout(x, 0.5, masks)  # draw 0 of the step, eager
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        a = ops.dropout(x, 0.5, masks)
+    with torch.cuda.graph(two):
+        b = ops.dropout(x, 0.5, masks)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = ops.dropout(x, 0.5, masks)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(c, ops.dropout(x, 0.5, (5, 3)))
+    for step in range(3):
+        for order in ((one, two), (two, one)):
+            for graph in order:
+                graph.replay()
+            assert torch.equal(a, ops.dropout(x, 0.5, (5, 4 * step + 1)))
+            assert torch.equal(b, ops.dropout(x, 0.5, (5, 4 * step + 2)))
+        if step == 0:
+            masks.advance()
+        else:
+            masks.state[1:].add_(4)  # as a step of four draws would

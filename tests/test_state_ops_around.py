@@ -326,3 +326,63 @@ def test_a_gradient_without_storage_is_a_zero_one(dtype, kind):
     grads = torch.autograd.grad(out, (x,) if r is None else (x, r), zero)
     for grad, of in zip(grads, (x, r)):
         assert grad.dtype == of.dtype and grad.shape == of.shape and not grad.any()
+
+
+# -- blocks that are computed twice ----------------------------------------------------------------
+
+def test_a_device_streams_draw_keeps_its_mask():
+    masks, x = ops.MaskStream(3, device="cpu"), torch.ones(300)
+    first, second = masks.next(), masks.next()
+    masks.advance()
+    third = masks.next()
+    masks.advance()
+    masks.load_state_dict({"seed": 9, "number": 5})
+    fourth = masks.next()
+    for draw, key in ((first, (3, 0)), (second, (3, 1)), (third, (3, 2)), (fourth, (9, 5)),
+                      (first, (3, 0))):
+        assert torch.equal(ops.dropout(x, 0.5, draw), ops.dropout(x, 0.5, key))
+    assert masks.state_dict() == {"seed": 9, "number": 6}
+
+
+def test_a_device_streams_draws_do_not_come_from_a_trace():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    masks, x = ops.MaskStream(3, device="cpu"), torch.ones(300)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        ops.dropout(mode.from_tensor(x), 0.5, masks)
+    graph = make_fx(lambda v: ops.dropout(v, 0.5, masks))(x)  # draw 1 of whatever the step begins with
+    assert torch.equal(ops.dropout(x, 0.5, masks), ops.dropout(x, 0.5, (3, 2)))
+    assert torch.equal(graph(x), ops.dropout(x, 0.5, (3, 1)))
+    masks.advance()
+    assert torch.equal(graph(x), ops.dropout(x, 0.5, (3, 4)))
+
+
+@pytest.mark.parametrize("device", [None, "cpu"])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_block_computed_twice_with_a_draw_from_outside(device, reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    masks = ops.MaskStream(3, device=device)
+    torch.manual_seed(0)
+    a, b = torch.nn.Linear(32, 48), torch.nn.Linear(48, 8)
+    x = torch.randn(16, 32, requires_grad=True)
+
+    def gradients(draw, twice):
+        def block(v):
+            return b(ops.dropout(a(v), 0.5, draw))
+        y = checkpoint(block, x, use_reentrant=reentrant) if twice else block(x)
+        if masks.state is not None:
+            masks.advance()  # before the backward pass
+        return torch.autograd.grad(y.pow(2).sum(), [x, *a.parameters(), *b.parameters()]) \
+            if not reentrant else _backward(y, [x, *a.parameters(), *b.parameters()])
+
+    def _backward(y, inputs):
+        for p in inputs:
+            p.grad = None
+        y.pow(2).sum().backward()
+        return [p.grad for p in inputs]
+
+    for number in range(3):
+        got, want = gradients(masks.next(), True), gradients((3, number), False)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
