@@ -6,6 +6,7 @@
 // same bits.
 #include <ATen/Parallel.h>
 #include <torch/extension.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/library.h>
 
 #include <vector>
@@ -327,6 +328,12 @@ TORCH_LIBRARY_IMPL(tpi, Autograd, m) { m.impl("dropout", &dropout_autograd); }
 
 void bind_dropout(py::module_& m) {
   m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
+  m.def("surroundings", [] {
+    const bool traced =
+        torch::jit::tracer::isTracing() ||
+        c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+    return (torch::autograd::get_current_graph_task_id() >= 0 ? 1 : 0) | (traced ? 2 : 0);
+  }, "bit 0: the caller runs inside a backward pass; bit 1: what it does is being recorded");
 }
 
 }  // namespace tpi

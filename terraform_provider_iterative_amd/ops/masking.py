@@ -15,7 +15,8 @@ Device tensors go through ``csrc/hip/dropout.hip``, host tensors through
 """
 from __future__ import annotations
 
-from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
+import threading
+from typing import Any, List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -42,8 +43,12 @@ class MaskStream:
         y = dropout(x, 0.1, masks)
 
     Each :func:`dropout` given the stream takes the next number.  A block that is computed twice
-    (activation checkpointing) has to draw the same mask both times: take ``masks.next()``
-    outside it and pass that.
+    (activation checkpointing) has to draw the same masks both times: take ``masks.next()``
+    outside it and pass that, or give the stream's contexts to the checkpoint::
+
+        y = checkpoint(block, x, use_reentrant=False, context_fn=masks.checkpoint_contexts)
+
+    Without either the second computation, which is a part of the backward pass, is refused.
 
     With ``device`` the seed and number are held there and read when a kernel runs, so that a
     captured graph draws new masks at every replay: call :meth:`advance` once per step, inside
@@ -63,25 +68,53 @@ class MaskStream:
             self._ahead = 0
             self._copies: dict = {}
 
-    def _copy(self) -> torch.Tensor:
+    def _copy(self, recorded: int) -> torch.Tensor:
         """What this step's draws refer to: a copy of the state, which advancing does not change.  One
         for each stream and each captured graph that draws, ordered before what it draws."""
         where = torch_hip().stream_and_capture(self.state.device.index) if self.state.is_cuda else 0
-        copy = None if _is_traced() else self._copies.get(where)
+        copy = None if recorded else self._copies.get(where)
         if copy is None:
             copy = self.state + 0  # a kernel
-            if type(copy) is torch.Tensor and not _is_traced():  # not a recording's
+            if type(copy) is torch.Tensor and not recorded:  # a fake one is not kept, either
                 self._copies[where] = copy
         return copy
 
+    def checkpoint_contexts(self) -> Tuple["_Frame", "_Frame"]:
+        """``context_fn`` of ``torch.utils.checkpoint.checkpoint(use_reentrant=False)``: the draws
+        that the block takes are kept, and given again when the backward pass computes it again."""
+        draws: List[Draw] = []
+        return _Frame(self, draws, False), _Frame(self, draws, True)
+
     def next(self) -> Draw:
+        """The stream's next draw (inside :meth:`checkpoint_contexts`' second context, the one that
+        the first one's block took here)."""
+        around = torch_ext().surroundings()
+        frames = [f for f in _frames.list if f.stream is self] if _frames.list else ()
+        for i in reversed(range(len(frames))):
+            if frames[i].again:
+                draw = frames[i].take()
+                frames = frames[i + 1:]  # blocks inside the one that is computed again
+                break
+        else:
+            if around & _IN_BACKWARD:
+                raise RuntimeError(
+                    "a block that the backward pass computes again would draw another mask: take its "
+                    "draw outside (draw = masks.next()), or checkpoint it with "
+                    "context_fn=masks.checkpoint_contexts")
+            draw = self._next(around & _RECORDED)
+        for frame in frames:
+            frame.draws.append(draw)
+        return draw
+
+    def _next(self, recorded: int) -> Draw:
         if self.state is not None:
+            copy = self._copy(recorded)
             self._ahead += 1
-            return Draw(0, self._ahead - 1, self._copy())
+            return Draw(0, self._ahead - 1, copy)
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             raise ValueError("a captured graph would repeat this stream's masks at every replay: "
                              "give MaskStream a device")
-        if not torch.compiler.is_dynamo_compiling() and _is_traced():
+        if recorded:
             raise ValueError("a traced program would repeat this stream's mask at every run: "
                              "give dropout a draw of its own")
         self.number += 1
@@ -111,9 +144,42 @@ class MaskStream:
             self.seed, self.number = seed, number
 
 
-def _is_traced() -> bool:
-    return torch._C._is_tracing() or \
-        torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+_IN_BACKWARD, _RECORDED = 1, 2  # torch_ext().surroundings()
+
+
+class _Frames(threading.local):
+    """The contexts that a thread is in, the innermost last."""
+
+    def __init__(self):
+        self.list: List["_Frame"] = []
+
+
+_frames = _Frames()
+
+
+class _Frame:
+    """A block that may be computed twice: ``draws`` are what it has taken from ``stream`` the first
+    time, and what it gets ``again``."""
+
+    def __init__(self, stream: MaskStream, draws: List[Draw], again: bool):
+        self.stream, self.draws, self.again = stream, draws, again
+
+    def __enter__(self) -> "_Frame":
+        self._given = 0
+        if not self.again:
+            self.draws.clear()
+        _frames.list.append(self)
+        return self
+
+    def __exit__(self, *exc: Any) -> None:
+        _frames.list.remove(self)
+
+    def take(self) -> Draw:
+        if self._given == len(self.draws):
+            raise RuntimeError("a block draws more masks when it is computed again (%d the first time)"
+                               % len(self.draws))
+        self._given += 1
+        return self.draws[self._given - 1]
 
 
 def _signed(value: int) -> int:
@@ -215,16 +281,18 @@ def dropout(x: torch.Tensor, p: float, draw: Union[MaskStream, Draw, Tuple[int, 
 
 class CounterDropout(torch.nn.Module):
     """:func:`dropout` as a layer: ``layer(x)`` or ``layer(x, residual)``.  Layers of a model
-    share one :class:`MaskStream`; in evaluation nothing is drawn or dropped."""
+    share one :class:`MaskStream`; in evaluation nothing is drawn or dropped.  ``draw`` takes the
+    place of the stream's next one (a layer in a block that is computed twice)."""
 
     def __init__(self, p: float, stream: MaskStream):
         super().__init__()
         keep_threshold(p)
         self.p, self.stream = float(p), stream
 
-    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                draw: Union[Draw, Tuple[int, int], None] = None) -> torch.Tensor:
         if self.training:
-            return dropout(x, self.p, self.stream, residual=residual)
+            return dropout(x, self.p, self.stream if draw is None else draw, residual=residual)
         return x if residual is None else dropout(x, 0.0, (0, 0), residual=residual)
 
     def extra_repr(self) -> str:

@@ -189,3 +189,59 @@ def test_draws_of_a_step_in_several_graphs_and_streams():
             masks.advance()
         else:
             masks.state[1:].add_(4)  # as a step of four draws would
+
+
+@pytest.mark.parametrize("device", [None, "cuda"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_checkpointed_layers_draw_the_same_masks_twice(device, captured):
+    from torch.utils.checkpoint import checkpoint
+
+    if captured and device is None:
+        pytest.skip("a stream without a device is refused in a capture")
+    masks = ops.MaskStream(9, device=device)
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Linear(64, 64), ops.CounterDropout(0.5, masks),
+                                torch.nn.Linear(64, 64), ops.CounterDropout(0.3, masks)).cuda()
+    x = torch.randn(32, 64, generator=torch.Generator().manual_seed(2)).cuda().requires_grad_(True)
+    inputs = [x, *model.parameters()]
+
+    def step():
+        y = checkpoint(model, x, use_reentrant=False, context_fn=masks.checkpoint_contexts)
+        if device:
+            masks.advance()
+        return torch.autograd.grad(y.pow(2).sum(), inputs)
+
+    def check(got, number):
+        a = ops.dropout(model[0](x), 0.5, (9, number))
+        b = ops.dropout(model[2](a), 0.3, (9, number + 1))
+        want = torch.autograd.grad(b.pow(2).sum(), inputs)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+        assert masks.state_dict()["number"] == number + 2
+
+    if not captured:
+        for number in (0, 2, 4):
+            check(step(), number)
+        return
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for replay in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        check(got, 2 + 2 * replay)
+
+
+def test_a_second_computation_without_the_contexts_is_refused():
+    from torch.utils.checkpoint import checkpoint
+
+    masks = ops.MaskStream(3, device="cuda")
+    x = torch.randn(64, device="cuda", requires_grad=True)
+    y = checkpoint(lambda v: ops.dropout(v, 0.5, masks).pow(2), x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match="computes again"):
+        y.sum().backward()
+    assert masks.state_dict()["number"] == 1

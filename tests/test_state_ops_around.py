@@ -386,3 +386,113 @@ def test_a_block_computed_twice_with_a_draw_from_outside(device, reentrant):
     for number in range(3):
         got, want = gradients(masks.next(), True), gradients((3, number), False)
         assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+class _Blocks(torch.nn.Module):
+    """Linear, CounterDropout, Linear, twice: the second block inside the first one's last layer."""
+
+    def __init__(self, masks):
+        super().__init__()
+        torch.manual_seed(0)
+        self.masks = masks
+        self.a, self.b, self.c, self.d = (torch.nn.Linear(24, 24) for _ in range(4))
+        self.one, self.two = ops.CounterDropout(0.5, masks), ops.CounterDropout(0.3, masks)
+
+    def inner(self, x):
+        return self.d(self.two(self.c(x)))
+
+    def outer(self, x, inner):
+        x = self.b(self.one(self.a(x), x))
+        return inner(x) + self.two(x)
+
+    def gradients(self, x, checkpoint, nested=False, times=1):
+        inner = (lambda v: checkpoint(self.inner, v)) if nested else self.inner
+        y = checkpoint(lambda v: self.outer(v, inner), x).pow(2).sum()
+        if self.masks.state is not None:
+            self.masks.advance()
+        for i in range(times):
+            out = torch.autograd.grad(y, [x, *self.parameters()], retain_graph=i + 1 < times)
+        return out
+
+
+@pytest.mark.parametrize("device", [None, "cpu"])
+@pytest.mark.parametrize("nested", [False, True])
+@pytest.mark.parametrize("compiled", [False, True])
+def test_checkpointed_layers_draw_the_same_masks_twice(device, nested, compiled):
+    from torch.utils.checkpoint import checkpoint
+
+    if compiled:
+        torch._dynamo.reset()
+    once, twice = (_Blocks(ops.MaskStream(3, device=device)) for _ in range(2))
+    x = torch.randn(16, 24, requires_grad=True)
+    if compiled:
+        twice.outer = torch.compile(twice.outer, backend="eager")
+    for step in range(3):
+        want = once.gradients(x, lambda f, v: f(v))
+        got = twice.gradients(x, lambda f, v: checkpoint(
+            f, v, use_reentrant=False, context_fn=twice.masks.checkpoint_contexts), nested, 1 + step)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+        assert twice.masks.state_dict() == once.masks.state_dict() == {"seed": 3, "number": 3 * step + 3}
+
+
+@pytest.mark.parametrize("device", [None, "cpu"])
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("compiled", [False, True])
+def test_a_second_computation_without_the_contexts_is_refused(device, reentrant, compiled):
+    from torch.utils.checkpoint import checkpoint
+
+    masks = ops.MaskStream(3, device=device)
+    block = torch.nn.Sequential(torch.nn.Linear(24, 24), ops.CounterDropout(0.5, masks),
+                                torch.nn.Linear(24, 24))
+    run = torch.compile(block, backend="eager") if compiled else block
+    y = checkpoint(run, torch.randn(4, 24, requires_grad=True), use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="computes again"):
+        y.sum().backward()
+    assert masks.state_dict()["number"] == 1
+    block(torch.randn(4, 24)).sum().backward()  # and the stream goes on
+    assert masks.state_dict()["number"] == 2
+
+
+def test_a_checkpointed_layer_with_a_draw():
+    from torch.utils.checkpoint import checkpoint
+
+    masks = ops.MaskStream(3)
+    layer, x = ops.CounterDropout(0.5, masks), torch.randn(40, requires_grad=True)
+    draw = masks.next()
+    y = checkpoint(lambda v: layer(v, draw=draw).pow(2), x, use_reentrant=True)
+    y.sum().backward()
+    dropped = ops.dropout(x.detach(), 0.5, (3, 0))
+    assert torch.equal(x.grad, ops.dropout(2 * dropped, 0.5, (3, 0))) and masks.number == 1
+    layer.eval()
+    assert layer(x, draw=draw) is x
+
+
+def test_a_block_that_draws_more_the_second_time_is_refused():
+    from torch.utils.checkpoint import checkpoint
+
+    masks, count = ops.MaskStream(3), []
+
+    def block(v):
+        count.append(0)
+        for _ in count:
+            v = ops.dropout(v, 0.5, masks)
+        return v.pow(2)
+
+    y = checkpoint(block, torch.ones(8, requires_grad=True), use_reentrant=False,
+                   context_fn=masks.checkpoint_contexts)
+    with pytest.raises(RuntimeError, match="draws more masks"):
+        y.sum().backward()
+    assert masks.number == 1
+
+
+def test_a_model_with_its_stream_can_be_copied_and_pickled():
+    import copy
+    import pickle
+
+    for device in (None, "cpu"):
+        model = _Blocks(ops.MaskStream(3, device=device))
+        model.one(torch.ones(8))
+        for other in (copy.deepcopy(model), pickle.loads(pickle.dumps(model))):
+            assert other.one.stream is other.masks is not model.masks
+            assert torch.equal(other.one(torch.ones(8)), ops.dropout(torch.ones(8), 0.5, (3, 1)))
+        assert model.masks.state_dict()["number"] == 1
