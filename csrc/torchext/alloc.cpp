@@ -24,6 +24,8 @@ at::Tensor empty_nogil(const std::vector<int64_t>& shape, const at::Tensor& like
 
 namespace tpi {
 
+uint64_t (*hip_stream_of)(int device);  // set by hip_stream.cpp
+
 static HipApi g_hip;
 
 const HipApi& hip_api() {

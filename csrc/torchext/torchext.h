@@ -1,12 +1,12 @@
 // Shared by the translation units of _tpi_torch.
 #pragma once
-#include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
 #include <stdexcept>
 #include <string>
 
 #include "../hip/tpi_hip.h"
+#include "streams.h"
 
 namespace tpi {
 
@@ -31,7 +31,8 @@ struct HipFailure : std::runtime_error {
 void hip_check(int rc, const char* what);
 
 inline uint64_t current_stream(c10::DeviceIndex device) {
-  return (uint64_t)c10::hip::getCurrentHIPStream(device).stream();
+  if (!hip_stream_of) throw HipFailure("this torch is not built for ROCm");
+  return hip_stream_of(device);
 }
 
 void bind_dropout(py::module_& m);

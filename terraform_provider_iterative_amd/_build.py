@@ -273,19 +273,22 @@ def build_stager(force: bool = False, verbose: bool = False) -> str:
 def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     """``_tpi_torch``: torch helpers that release the GIL, torch operators and their launches
     (``csrc/torchext``; host code against torch's own headers and libraries, same C++ ABI)."""
-    srcs = _sources("torchext/*.cpp")
-    if not srcs:
-        return ""
     import torch
 
     import sysconfig
+
+    # without ROCm (a control-plane host) it serves host tensors only
+    rocm = torch.version.hip is not None
+    srcs = [s for s in _sources("torchext/*.cpp") if rocm or not s.endswith("hip_stream.cpp")]
+    if not srcs:
+        return ""
 
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     tl = torch_lib_dir()
     cxx = os.environ.get("CXX", "g++")
     flags = [cxx, "-O3", "-std=c++17", "-fPIC", "-Wall", "-pthread",
-             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",  # c10's stream of a device
-             "-isystem", os.path.join(os.path.dirname(ROCM_LIB), "include"),
+             *(["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",  # what c10's stream of a device asks for
+                "-isystem", os.path.join(os.path.dirname(ROCM_LIB), "include")] if rocm else []),
              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
              "-DTORCH_EXTENSION_NAME=_tpi_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
              "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
@@ -294,7 +297,8 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     headers = _sources("torchext/*.h", "common/*.h", "hip/tpi_hip.h") + [
         os.path.join(os.path.dirname(torch.__file__), "version.py")]
     link = [cxx, "-shared", "-fPIC", "-pthread", "@OBJS@", "-L" + tl, "-Wl,-rpath," + tl, "-lc10",
-            "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-o", "@OUT@"]
+            *(["-lc10_hip"] if rocm else []), "-ltorch", "-ltorch_cpu", "-ltorch_python",
+            "-o", "@OUT@"]
     # torch's headers take a minute per source
     return _build_objects(TORCH_EXT, flags, srcs, link, headers, "torchext_", len(srcs), force,
                           verbose)

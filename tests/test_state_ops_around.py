@@ -496,3 +496,43 @@ def test_a_model_with_its_stream_can_be_copied_and_pickled():
             assert other.one.stream is other.masks is not model.masks
             assert torch.equal(other.one(torch.ones(8)), ops.dropout(torch.ones(8), 0.5, (3, 1)))
         assert model.masks.state_dict()["number"] == 1
+
+
+# -- builds ----------------------------------------------------------------------------------------
+
+def test_the_host_operators_build_without_rocm(tmp_path, monkeypatch):
+    """With a torch that is not built for ROCm, and no ROCm there, _tpi_torch serves host tensors."""
+    import os
+    import subprocess
+    import sys
+
+    from terraform_provider_iterative_amd import _build
+
+    target = str(tmp_path / os.path.basename(_build.TORCH_EXT))
+    monkeypatch.setattr(torch.version, "hip", None)
+    monkeypatch.setattr(_build, "TORCH_EXT", target)
+    monkeypatch.setattr(_build, "LIB", str(tmp_path))
+    monkeypatch.setattr(_build, "ROCM_LIB", str(tmp_path / "rocm" / "lib"))
+    assert _build.build_torch_ext() == target
+    needed = subprocess.run(["readelf", "-d", target], capture_output=True, text=True, check=True).stdout
+    assert "libtorch_cpu" in needed and "hip" not in needed
+    script = """if True:
+        import importlib.util, sys, torch
+        spec = importlib.util.spec_from_file_location("_tpi_torch", sys.argv[1])
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        from terraform_provider_iterative_amd import ops
+        from terraform_provider_iterative_amd.ops import _loader
+        _loader._torch_ext = module
+        out = ops.dropout(torch.ones(100, requires_grad=True), 0.5, ops.MaskStream(3))
+        out.sum().backward()
+        try:
+            module.stream_and_capture(0)
+        except ops.HipError as error:
+            print(int(out.sum()), error)
+    """
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", script, target], capture_output=True, text=True,
+                         env=dict(os.environ, PYTHONPATH=root), timeout=120)
+    want = int(ops.dropout(torch.ones(100), 0.5, (3, 0)).sum())
+    assert res.stdout.startswith("%d this torch is not built for ROCm" % want), res.stdout + res.stderr
