@@ -286,7 +286,9 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> str:
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
     tl = torch_lib_dir()
     cxx = os.environ.get("CXX", "g++")
-    flags = [cxx, "-O3", "-std=c++17", "-fPIC", "-Wall", "-pthread",
+    # at::parallel_for is a serial loop in sources compiled without OpenMP.  Its runtime is not linked:
+    # the symbols come from the one that torch's libraries bring, and there is no second one.
+    flags = [cxx, "-O3", "-std=c++17", "-fPIC", "-Wall", "-pthread", "-fopenmp",
              *(["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",  # what c10's stream of a device asks for
                 "-isystem", os.path.join(os.path.dirname(ROCM_LIB), "include")] if rocm else []),
              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),

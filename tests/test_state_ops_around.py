@@ -4,6 +4,7 @@ import pytest
 import torch
 import torch.distributed as dist
 
+from state_oracles import keep_mask
 from terraform_provider_iterative_amd import ops
 from terraform_provider_iterative_amd.checkpoint import TrainingState
 
@@ -536,3 +537,42 @@ def test_the_host_operators_build_without_rocm(tmp_path, monkeypatch):
                          env=dict(os.environ, PYTHONPATH=root), timeout=120)
     want = int(ops.dropout(torch.ones(100), 0.5, (3, 0)).sum())
     assert res.stdout.startswith("%d this torch is not built for ROCm" % want), res.stdout + res.stderr
+
+
+@pytest.mark.parametrize("shape", [(3 * (1 << 15) + 5,), (7, 41, 1031)])
+@pytest.mark.parametrize("turned", [False, True])
+def test_host_dropout_on_several_threads(shape, turned):
+    """Ranges are split where they fall, inside a block of the generator and inside a row."""
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(1))
+    x = x.t() if turned and x.dim() == 2 else x.transpose(0, -1) if turned else x
+    r = torch.randn(x.shape, generator=torch.Generator().manual_seed(2)).half().float()
+    threads = torch.get_num_threads()
+    try:
+        results = []
+        for count in (1, 2, 3, 5):
+            torch.set_num_threads(count)
+            results.append(ops.dropout(x, 0.3, KEY, residual=r))
+    finally:
+        torch.set_num_threads(threads)
+    assert all(torch.equal(out, results[0]) for out in results)
+    kept = torch.tensor(keep_mask(range(x.numel()), 0.3, *KEY)).reshape(x.shape)
+    product = torch.where(kept, x.double() * (2 ** 32 / int(round(0.7 * 2 ** 32))), 0.0)
+    # in 32 bits: the scale, the product and the sum are each rounded by half a step
+    bound = 3 * 2.0 ** -24 * (product.abs() + r.double().abs())
+    assert ((results[-1].double() - product - r.double()).abs() <= bound).all()
+
+
+def test_the_host_operators_are_built_for_torchs_threads():
+    """at::parallel_for compiled without OpenMP runs on one; the runtime is torch's, not a second."""
+    import subprocess
+
+    from terraform_provider_iterative_amd import _build
+
+    if not torch.__config__.parallel_info().count("ATen parallel backend: OpenMP"):
+        pytest.skip("torch itself does not use OpenMP")
+    _build.build_torch_ext()
+    names = subprocess.run(["nm", "-D", "--undefined-only", _build.TORCH_EXT], capture_output=True,
+                           text=True, check=True).stdout
+    needed = subprocess.run(["readelf", "-d", _build.TORCH_EXT], capture_output=True, text=True,
+                            check=True).stdout
+    assert "GOMP_parallel" in names and "omp" not in needed
