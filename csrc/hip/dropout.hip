@@ -339,8 +339,7 @@ int launch_rows(const tpi_dropout_args& a, hipStream_t stream) {
   const uint32_t grid = finish(k);
   if (!grid) return tpi_fail("dropout: tensor too large");
   const auto kernel = last ? k_dropout_rows<IN, OUT, RES, false> : k_dropout_rows<IN, OUT, RES, true>;
-  kernel<<<grid, kThreads, 0, stream>>>(k);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(kernel, grid, kThreads, stream, k));
   return 0;
 }
 
@@ -362,8 +361,8 @@ int launch_tiles(const tpi_dropout_args& a, int along, int across, hipStream_t s
   t.row.per_row = (uint64_t)(t.across + 7) / 8;
   const uint32_t grid = finish(t.row);
   if (!grid) return tpi_fail("dropout: tensor too large");
-  k_dropout_tiles<IN, OUT, RES><<<grid, kThreads, 0, stream>>>(t);
-  TPI_HIP(hipGetLastError());
+  const auto kernel = k_dropout_tiles<IN, OUT, RES>;
+  TPI_HIP(tpi_launch(kernel, grid, kThreads, stream, t));
   return 0;
 }
 
@@ -387,8 +386,8 @@ int launch(const tpi_dropout_args& a, hipStream_t stream) {
   for (int d = 0; d < a.ndim; ++d) total *= (uint64_t)a.sizes[d];
   const uint64_t want = (total + kThreads - 1) / kThreads;
   const uint32_t grid = (uint32_t)(want < 65536 ? want : 65536);
-  k_dropout_strided<IN, OUT, RES><<<grid, kThreads, 0, stream>>>(a, total);
-  TPI_HIP(hipGetLastError());
+  const auto kernel = k_dropout_strided<IN, OUT, RES>;
+  TPI_HIP(tpi_launch(kernel, grid, kThreads, stream, a, total));
   return 0;
 }
 

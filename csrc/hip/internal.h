@@ -3,9 +3,25 @@
 #include <hip/hip_runtime.h>
 
 #include <string>
+#include <tuple>
 
 // Sets the thread's tpi_last_error() text; returns -1.
 int tpi_fail(const std::string& what);
+
+// Launches a kernel and returns that launch's own error.  hipGetLastError() behind <<<>>> also returns
+// what some earlier call of this thread has left there, after its caller has dealt with it: work
+// that has begun would be reported as failed, and of several launches the rest left out.
+template <typename... P, typename... A>
+static inline hipError_t tpi_launch(void (*kernel)(P...), dim3 grid, uint32_t block,
+                                    hipStream_t stream, A... a) {
+  std::tuple<P...> args(a...);
+  return std::apply(
+      [&](P&... each) {
+        void* list[] = {(void*)&each...};
+        return hipLaunchKernel((const void*)kernel, grid, dim3(block), list, 0, stream);
+      },
+      args);
+}
 
 #define TPI_HIP(expr)                                                              \
   do {                                                                             \

@@ -623,9 +623,8 @@ extern "C" {
 int tpi_pages_copy(const tpi_pages* p, const void* src, const void* dst, int64_t n, int wide,
                    uint64_t stream) {
   if (n <= 0) return 0;
-  k_copy<<<dim3(p->chunks, rows_of(n)), kBlock, 0, (hipStream_t)stream>>>(*p, src, dst, n,
-                                                                           wide & 1);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(k_copy, dim3(p->chunks, rows_of(n)), kBlock, (hipStream_t)stream, *p, src, dst, n,
+                     wide & 1));
   return 0;
 }
 
@@ -635,11 +634,10 @@ int tpi_pages_fork(const tpi_pages* p, const void* src, const void* dst, int64_t
   if (n > p->slots) return tpi_fail("fork: more destinations than slots");
   hipStream_t s = (hipStream_t)stream;
   const auto reserve = few(p, n) ? k_reserve_few<true> : k_reserve<true>;
-  reserve<<<1, kPlan, 0, s>>>(*p, src, dst, (int)n, wide & 1, nullptr, false, 0);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(reserve, 1, kPlan, s, *p, src, dst, (int)n, wide & 1, nullptr, false, 0));
   const int spans = (p->width + kRowSpan - 1) / kRowSpan;
-  k_fork<<<dim3(spans + p->chunks, rows_of(n)), kBlock, 0, s>>>(*p, src, dst, n, wide & 1, spans);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(k_fork, dim3(spans + p->chunks, rows_of(n)), kBlock, s, *p, src, dst, n, wide & 1,
+                     spans));
   return 0;
 }
 
@@ -648,9 +646,8 @@ int tpi_pages_extend(const tpi_pages* p, const void* slots, int64_t n, int wide,
   if (n <= 0) return 0;
   if (n > p->slots) return tpi_fail("extend: more sequences than slots");
   const auto reserve = few(p, n) ? k_reserve_few<false> : k_reserve<false>;
-  reserve<<<1, kPlan, 0, (hipStream_t)stream>>>(*p, slots, nullptr, (int)n, wide & 1, more,
-                                                (wide & 2) != 0, each);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(reserve, 1, kPlan, (hipStream_t)stream, *p, slots, nullptr, (int)n, wide & 1, more,
+                     (wide & 2) != 0, each));
   return 0;
 }
 
@@ -660,26 +657,21 @@ int tpi_pages_free(const tpi_pages* p, const void* slots, int64_t n, int wide, u
   hipStream_t s = (hipStream_t)stream;
   const bool many = n > kPlan;  // up to here a workgroup's own look at all slots is 4 loads a thread
   if (many) {
-    k_free_check<<<1, kPlan, 0, s>>>(*p, slots, n, wide & 1);
-    TPI_HIP(hipGetLastError());
+    TPI_HIP(tpi_launch(k_free_check, 1, kPlan, s, *p, slots, n, wide & 1));
   }
-  k_free<<<(uint32_t)n, kBlock, 0, s>>>(*p, slots, n, wide & 1, many);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(k_free, (uint32_t)n, kBlock, s, *p, slots, n, wide & 1, many));
   return 0;
 }
 
 int tpi_pages_compact(const tpi_pages* p, int clear, uint64_t stream) {
   hipStream_t s = (hipStream_t)stream;
-  k_plan<<<1, kPlan, 0, s>>>(*p, clear != 0);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(k_plan, 1, kPlan, s, *p, clear != 0));
   const int64_t table = ((int64_t)p->slots * p->width + 4 * kBlock - 1) / (4 * kBlock);
   const int chunks = (int)rows_of(p->chunks);
   const int spans = (int)(((table < 256 ? table : 256) + chunks - 1) / chunks);
-  k_compact<<<dim3(spans + spread(p), chunks), kBlock, 0, s>>>(*p, spans);
-  TPI_HIP(hipGetLastError());
+  TPI_HIP(tpi_launch(k_compact, dim3(spans + spread(p), chunks), kBlock, s, *p, spans));
   if (clear) {
-    k_clear<<<dim3(spread(p), chunks), kBlock, 0, s>>>(*p);
-    TPI_HIP(hipGetLastError());
+    TPI_HIP(tpi_launch(k_clear, dim3(spread(p), chunks), kBlock, s, *p));
   }
   return 0;
 }

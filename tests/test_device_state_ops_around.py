@@ -245,3 +245,30 @@ def test_a_second_computation_without_the_contexts_is_refused():
     with pytest.raises(RuntimeError, match="computes again"):
         y.sum().backward()
     assert masks.state_dict()["number"] == 1
+
+
+# -- errors, streams, memory -----------------------------------------------------------------------
+
+def test_an_earlier_calls_error_is_not_a_launchs():
+    """What another caller has left in the runtime's last error neither fails an operation nor leaves
+    out a part of it."""
+    import ctypes
+
+    from terraform_provider_iterative_amd import _build
+
+    runtime = ctypes.CDLL(_build.HIP_SO)  # finds the runtime that the library is linked to
+    x = torch.ones(1000, device="cuda")
+    pool = ops.PagePool([torch.ones(32, 64, device="cuda")], 4, 8, 8)
+    slots = [torch.tensor(v, device="cuda") for v in ([0], [1, 2], [0, 0])]
+    torch.cuda.synchronize()
+    calls = [lambda: ops.dropout(x, 0.5, (1, 2)), lambda: pool.extend(slots[0], 7),
+             lambda: pool.fork(slots[2], slots[1]), lambda: pool.free(slots[0]),
+             lambda: pool.copy(slots[0], slots[1][:1]), lambda: pool.compact(clear=True)]
+    for call in calls:
+        assert runtime.hipSetDevice(1 << 20) != 0  # refused, and remembered
+        try:
+            call()
+        finally:
+            assert runtime.hipGetLastError() != 0  # still there for whoever asks
+    assert pool.status() == {"pages": 32, "free": 29, "live": 3, "error": None}
+    assert pool.lengths.tolist() == [0, 7, 7] + [0] * 5
