@@ -1,5 +1,5 @@
 // Launches of csrc/hip/pages.hip on the current stream of a pool's device (ops/paging.py); the
-// pool's description is the bytes of a tpi_pages.
+// pool's description is the bytes of a tpi_pages.  Each returns the stream.
 #include <string.h>
 
 #include "torchext.h"
@@ -30,12 +30,14 @@ void bind_pages(py::module_& m) {
     const Pool pool(raw, device);
     hip_check(hip_api().pages_copy(&pool.p, address(src), address(dst), n, wide, pool.stream),
               "copy");
+    return pool.stream;
   });
   m.def("pages_fork", [](const py::bytes& raw, int device, uintptr_t src, uintptr_t dst,
                          int64_t n, int wide) {
     const Pool pool(raw, device);
     hip_check(hip_api().pages_fork(&pool.p, address(src), address(dst), n, wide, pool.stream),
               "fork");
+    return pool.stream;
   });
   m.def("pages_extend", [](const py::bytes& raw, int device, uintptr_t slots, int64_t n, int wide,
                            uintptr_t more, int64_t each) {
@@ -43,14 +45,17 @@ void bind_pages(py::module_& m) {
     hip_check(hip_api().pages_extend(&pool.p, address(slots), n, wide, address(more), each,
                                      pool.stream),
               "extend");
+    return pool.stream;
   });
   m.def("pages_free", [](const py::bytes& raw, int device, uintptr_t slots, int64_t n, int wide) {
     const Pool pool(raw, device);
     hip_check(hip_api().pages_free(&pool.p, address(slots), n, wide, pool.stream), "free");
+    return pool.stream;
   });
   m.def("pages_compact", [](const py::bytes& raw, int device, int clear) {
     const Pool pool(raw, device);
     hip_check(hip_api().pages_compact(&pool.p, clear, pool.stream), "compact");
+    return pool.stream;
   });
 }
 

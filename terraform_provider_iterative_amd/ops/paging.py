@@ -119,6 +119,9 @@ class PagePool:
                                      self._chunk)]
         self._args = _POOL.pack(*at, self.pages, self.slots, self.width, self.page_tokens,
                                 self._chunks, 0)
+        self._streams = set()  # that use the memory: the one that it was allocated on, to begin with
+        if self._on_device:
+            self._streams.add(torch_hip().stream_and_capture(self.device.index)[0])
         self._write_books(np.full((self.slots, self.width), -1, np.int32),
                           np.zeros(self.slots, np.int32))
 
@@ -245,7 +248,11 @@ class PagePool:
 
     def _enqueue(self, name: str, *args) -> None:
         if self._on_device:
-            getattr(torch_hip(), "pages_" + name)(self._args, self.device.index, *args)
+            stream = getattr(torch_hip(), "pages_" + name)(self._args, self.device.index, *args)
+            if stream not in self._streams:  # a pool that is dropped keeps its memory until it is done
+                self._streams.add(stream)
+                for t in (self.meta, self._scratch, self._chunk, *self.tensors):
+                    t.record_stream(torch.cuda.current_stream(self.device))
             return
         getattr(native(), "pages_" + name)(self._args, *args)
         self.check()

@@ -272,3 +272,28 @@ def test_an_earlier_calls_error_is_not_a_launchs():
             assert runtime.hipGetLastError() != 0  # still there for whoever asks
     assert pool.status() == {"pages": 32, "free": 29, "live": 3, "error": None}
     assert pool.lengths.tolist() == [0, 7, 7] + [0] * 5
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_dropped_pools_memory_waits_for_a_side_stream(captured):
+    """Nothing that a pool allocated, nor its tensors, is given to another tensor while work that the
+    pool has enqueued on a side stream may still use it."""
+    side = torch.cuda.Stream()
+    pool = ops.PagePool([torch.ones(5000, 1 << 12, device="cuda")], 4, 16, 5000)
+    pool.extend([0, 1], [8000, 8000])
+    pool.free([0])
+    held = {t.data_ptr(): t.numel() for t in (pool.meta, pool._scratch, pool._chunk, pool.tensors[0])}
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            pool.compact()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # some tenths of a second
+        pool.compact(clear=True)
+    del pool
+    other = [torch.empty(n, dtype=torch.int32 if n < 1 << 24 else torch.float32, device="cuda")
+             for n in held.values()]
+    assert not side.query()
+    assert not set(held) & {t.data_ptr() for t in other}
+    torch.cuda.synchronize()
