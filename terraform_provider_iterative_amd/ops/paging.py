@@ -125,6 +125,22 @@ class PagePool:
         self._write_books(np.full((self.slots, self.width), -1, np.int32),
                           np.zeros(self.slots, np.int32))
 
+    # The kernels' arguments are addresses: a deep or unpickled copy is built around its own tensors
+    # and books, a shallow one is another name for the same.
+    def __reduce__(self):
+        return PagePool._rebuilt, (self.tensors, self.page_tokens, self.slots, self.width, self.meta)
+
+    def __copy__(self) -> "PagePool":
+        out = object.__new__(type(self))
+        out.__dict__.update(self.__dict__)
+        return out
+
+    @staticmethod
+    def _rebuilt(tensors, page_tokens, slots, width, meta) -> "PagePool":
+        pool = PagePool(tensors, page_tokens, slots, width)
+        pool.meta.copy_(meta)
+        return pool
+
     def _lay_out_tensors(self) -> None:
         parts, layouts = [], {}  # tensors mostly share one layout: cut it once
         for t in self.tensors:

@@ -576,3 +576,54 @@ def test_the_host_operators_are_built_for_torchs_threads():
     needed = subprocess.run(["readelf", "-d", _build.TORCH_EXT], capture_output=True, text=True,
                             check=True).stdout
     assert "GOMP_parallel" in names and "omp" not in needed
+
+
+# -- pools ---------------------------------------------------------------------------------------
+
+def _pool():
+    kv = torch.arange(2.0 * 10 * 4).reshape(2, 10, 4)
+    pool = ops.PagePool(list(kv.unbind(0)), 4, 3, 5)
+    pool.extend([0, 2], [9, 3])
+    return pool
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "state_dict"])
+def test_a_copied_pool_has_books_and_pages_of_its_own(how):
+    import copy
+    import pickle
+
+    pool = _pool()
+    books, data = pool.meta.clone(), [t.clone() for t in pool.tensors]
+    if how == "pickle":
+        other = pickle.loads(pickle.dumps(pool))
+    elif how == "deepcopy":
+        other = copy.deepcopy(pool)
+    else:  # as an attribute of a module that is copied
+        module = torch.nn.Linear(2, 2)
+        module.cache = pool
+        other = copy.deepcopy(module).cache
+    assert torch.equal(other.meta, books) and other.width == 5
+    assert all(torch.equal(a, b) for a, b in zip(other.tensors, data))
+    other.fork([0], [1])
+    other.copy([0], [9])
+    other.free([2])
+    assert torch.equal(pool.meta, books) and all(torch.equal(a, b) for a, b in zip(pool.tensors, data))
+    want = _pool()
+    want.fork([0], [1])
+    want.copy([0], [9])
+    want.free([2])
+    assert torch.equal(other.meta, want.meta)
+    assert all(torch.equal(a, b) for a, b in zip(other.tensors, want.tensors))
+    del pool
+    other.compact(clear=True)
+    want.compact(clear=True)
+    assert torch.equal(other.meta, want.meta)
+
+
+def test_a_shallow_copy_is_the_same_pool():
+    import copy
+
+    pool = _pool()
+    other = copy.copy(pool)
+    other.free([0])
+    assert other.meta is pool.meta and pool.status()["live"] == 1
