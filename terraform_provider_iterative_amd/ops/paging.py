@@ -206,7 +206,8 @@ class PagePool:
     # -- books from the host ------------------------------------------------------------------
     def bind(self, table, lengths) -> "PagePool":
         """Take over sequences whose pages are already in the tensors: ``table`` ``[slots, <=
-        width]`` and ``lengths`` ``[slots]``.  Waits for the device."""
+        width]`` and ``lengths`` ``[slots]``.  Sequences may share full pages; a partial last page is
+        written by the next extension, so no other entry may name it.  Waits for the device."""
         table = torch.as_tensor(table).cpu().numpy().astype(np.int64)
         lengths = torch.as_tensor(lengths).cpu().numpy().astype(np.int64)
         if table.ndim != 2 or table.shape[0] != self.slots or table.shape[1] > self.width \
@@ -221,6 +222,10 @@ class PagePool:
             raise ValueError("a page of the table is out of range")
         books = np.full((self.slots, self.width), -1, np.int32)
         books[:, :table.shape[1]] = np.where(held, table, -1)
+        part = (lengths % self.page_tokens != 0).nonzero()[0]
+        named = np.bincount(books[books >= 0], minlength=self.pages)
+        if (named[books[part, lengths[part] // self.page_tokens]] > 1).any():
+            raise ValueError("a partial last page is named twice: give each sequence a copy")
         self._write_books(books, lengths.astype(np.int32))
         return self
 

@@ -627,3 +627,19 @@ def test_a_shallow_copy_is_the_same_pool():
     other = copy.copy(pool)
     other.free([0])
     assert other.meta is pool.meta and pool.status()["live"] == 1
+
+
+def test_bind_refuses_a_partial_page_of_two_sequences():
+    """Either would go on writing in it; full pages may be shared, and a partial one of one sequence."""
+    pool = ops.PagePool([torch.zeros(10, 4)], 4, 3, 5)
+    before = pool.meta.clone()
+    for table, lengths in (([[1, 2], [1, 2], [0, 0]], [7, 7, 0]),   # partial in both
+                           ([[1, 2], [2, 3], [0, 0]], [7, 8, 0]),   # partial in one, full in the other
+                           ([[1, 1], [2, 3], [0, 0]], [5, 8, 0])):  # both in one sequence
+        with pytest.raises(ValueError, match="partial"):
+            pool.bind(table, lengths)
+        assert torch.equal(pool.meta, before)
+    pool.bind([[1, 2], [1, 3], [1, 4]], [7, 5, 8])
+    assert pool.refs.tolist() == [0, 3, 1, 1, 1] + [0] * 5
+    pool.bind([[1, 2], [1, 2], [1, 2]], [8, 8, 4])
+    assert pool.refs.tolist() == [0, 3, 2] + [0] * 7
