@@ -89,11 +89,11 @@ class MaskStream:
         """The stream's next draw (inside :meth:`checkpoint_contexts`' second context, the one that
         the first one's block took here)."""
         around = torch_ext().surroundings()
-        frames = [f for f in _frames.list if f.stream is self] if _frames.list else ()
-        for i in reversed(range(len(frames))):
-            if frames[i].again:
-                draw = frames[i].take()
-                frames = frames[i + 1:]  # blocks inside the one that is computed again
+        uses = [use for use in _frames.uses if use.frame.stream is self] if _frames.uses else ()
+        for i in reversed(range(len(uses))):
+            if uses[i].frame.again:
+                draw = uses[i].take()
+                uses = uses[i + 1:]  # blocks inside the one that is computed again
                 break
         else:
             if around & _IN_BACKWARD:
@@ -102,8 +102,8 @@ class MaskStream:
                     "draw outside (draw = masks.next()), or checkpoint it with "
                     "context_fn=masks.checkpoint_contexts")
             draw = self._next(around & _RECORDED)
-        for frame in frames:
-            frame.draws.append(draw)
+        for use in uses:
+            use.frame.draws.append(draw)
         return draw
 
     def _next(self, recorded: int) -> Draw:
@@ -151,7 +151,7 @@ class _Frames(threading.local):
     """The contexts that a thread is in, the innermost last."""
 
     def __init__(self):
-        self.list: List["_Frame"] = []
+        self.uses: List["_Use"] = []
 
 
 _frames = _Frames()
@@ -165,21 +165,29 @@ class _Frame:
         self.stream, self.draws, self.again = stream, draws, again
 
     def __enter__(self) -> "_Frame":
-        self._given = 0
         if not self.again:
             self.draws.clear()
-        _frames.list.append(self)
+        _frames.uses.append(_Use(self))
         return self
 
     def __exit__(self, *exc: Any) -> None:
-        _frames.list.remove(self)
+        last = max(i for i, use in enumerate(_frames.uses) if use.frame is self)
+        del _frames.uses[last]
+
+
+class _Use:
+    """One pass through a frame's block: every backward pass over a graph makes one of its own."""
+
+    def __init__(self, frame: _Frame):
+        self.frame, self.given = frame, 0
 
     def take(self) -> Draw:
-        if self._given == len(self.draws):
+        draws = self.frame.draws
+        if self.given == len(draws):
             raise RuntimeError("a block draws more masks when it is computed again (%d the first time)"
-                               % len(self.draws))
-        self._given += 1
-        return self.draws[self._given - 1]
+                               % len(draws))
+        self.given += 1
+        return draws[self.given - 1]
 
 
 def _signed(value: int) -> int:

@@ -643,3 +643,27 @@ def test_bind_refuses_a_partial_page_of_two_sequences():
     assert pool.refs.tolist() == [0, 3, 1, 1, 1] + [0] * 5
     pool.bind([[1, 2], [1, 2], [1, 2]], [8, 8, 4])
     assert pool.refs.tolist() == [0, 3, 2] + [0] * 7
+
+
+def test_two_threads_compute_one_block_again_at_once():
+    """Each backward pass over a graph is given the block's draws from the first on."""
+    import threading
+
+    masks = ops.MaskStream(3)
+    first, again = masks.checkpoint_contexts()
+    with first:
+        drawn = [masks.next() for _ in range(4)]
+    barrier, got = threading.Barrier(2, timeout=60), [[], []]
+
+    def compute(out):
+        with again:
+            for _ in drawn:
+                barrier.wait()
+                out.append(masks.next())
+
+    threads = [threading.Thread(target=compute, args=(out,)) for out in got]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got[0] == got[1] == drawn and masks.number == 4
