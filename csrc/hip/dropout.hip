@@ -216,8 +216,8 @@ struct TileArgs {
 // Tiles of 8 elements along the index, which are one generator block, by 8 across it, which are
 // neighbours in memory.  Every block of the view is whole or cut at the dimension's end (the
 // host has checked: all steps of the index but this one are multiples of 8).  Lanes lie across,
-// so that their accesses join to whole lines.  16M bf16 elements, channels last: 16.2 us, 127 with
-// a thread and a block of the generator per element (contiguous: 13.3).
+// so that their accesses join to whole lines.  16M bf16 elements, channels last: 15.6 us, 123 with
+// a thread and a block of the generator per element (contiguous: 13.2).
 template <int IN, int OUT, bool RES>
 __global__ __launch_bounds__(kThreads) void k_dropout_tiles(TileArgs t) {
   typedef typename Elem<IN>::type TI;

@@ -1,7 +1,7 @@
 // Counter-based dropout as a differentiable torch operator (ops/masking.py): the host side of
 // every call -- output, view walked, launch -- and its autograd node, without Python in either
-// direction: a forward and a backward pass cost the host 47 us (120 as Python functions; torch's own
-// dropout and addition 55, an addition alone 34).
+// direction: a forward and a backward pass cost the host 53 us where torch's own dropout and addition
+// cost it 61 and an addition alone 40 (as Python functions they cost 120 where this costs 47).
 // Device tensors go to tpi_dropout (csrc/hip/dropout.hip); host tensors are computed here, to the
 // same bits.
 #include <ATen/Parallel.h>

@@ -61,7 +61,7 @@ class PagePool:
     """The pages of ``tensors`` and the ``slots`` sequences that hold them.
 
     ``tensors``: one or more tensors of one device whose first dimension is the page, all with the
-    same number of pages; a page's bytes are one contiguous run, or several with one stride
+    same number of pages and none sharing memory; a page's bytes are one contiguous run, or several with one stride
     between them (``[heads, pages, ...]`` storage seen pages first).  ``page_tokens``: tokens
     of a page.  ``width``: pages that one sequence can have (default: all).
 
