@@ -164,7 +164,8 @@ void check_args(TPI_DROPOUT_ARGS) {
   const at::ScalarType type = x.scalar_type();
   TORCH_CHECK_TYPE(type_ok(type) && type_ok(dtype) &&
                        (type == dtype || type == at::kFloat || dtype == at::kFloat) &&
-                       (!residual || residual->scalar_type() == dtype),
+                       (!residual || (residual->scalar_type() == dtype &&
+                                      (type == dtype || dtype == at::kFloat))),
                    "dropout: unsupported types");
   TORCH_CHECK_VALUE(!residual || (residual->sizes() == x.sizes() && residual->device() == x.device()),
                     "dropout: the residual must have x's shape and device");

@@ -238,6 +238,7 @@ def test_the_operators_own_refusals():
     assert torch.equal(torch.ops.tpi.dropout(**good), ops.dropout(x, 0.5, (1, 2)))
     for bad in (dict(x=x.double()), dict(dtype=torch.float64), dict(dtype=torch.int16),
                 dict(x=x.half(), dtype=torch.bfloat16), dict(residual=x.half()),
+                dict(residual=x.half(), dtype=torch.float16),
                 dict(residual=torch.ones(4)), dict(threshold=-1), dict(threshold=(1 << 32) + 1),
                 dict(number=-1), dict(first=-1), dict(strides=[1]), dict(state=torch.zeros(2)),
                 dict(state=torch.zeros(3, dtype=torch.int64)),
