@@ -81,8 +81,7 @@ struct TpiRange {
 #define HIP_OK(expr)                                                                    \
   do {                                                                                  \
     hipError_t e_ = (expr);                                                             \
-    if (e_ != hipSuccess)                                                               \
-      return tpi_fail(std::string(#expr) + ": " + hipGetErrorString(e_));               \
+    if (e_ != hipSuccess) return tpi_hip_fail(#expr, e_);                               \
   } while (0)
 
 // Progressive pinning of a (large, existing) host region: a toucher thread faults the pages

@@ -23,10 +23,18 @@ static inline hipError_t tpi_launch(void (*kernel)(P...), dim3 grid, uint32_t bl
       args);
 }
 
-#define TPI_HIP(expr)                                                              \
-  do {                                                                             \
-    hipError_t e_ = (expr);                                                        \
-    if (e_ != hipSuccess) return tpi_fail(std::string(#expr) + ": " + hipGetErrorString(e_)); \
+// Sets tpi_last_error() to a failed call's; returns -1.  The runtime remembers the error too, and a later
+// look at hipGetLastError() (torch's, behind its own kernels) would take it for its own: it is
+// reported here, and taken back there.
+static inline int tpi_hip_fail(const char* what, hipError_t error) {
+  (void)hipGetLastError();
+  return tpi_fail(std::string(what) + ": " + hipGetErrorString(error));
+}
+
+#define TPI_HIP(expr)                                       \
+  do {                                                      \
+    hipError_t e_ = (expr);                                 \
+    if (e_ != hipSuccess) return tpi_hip_fail(#expr, e_);   \
   } while (0)
 
 // SDMA device -> host copies (sdma.cpp).  tpi_sdma_open returns nullptr when the lanes are

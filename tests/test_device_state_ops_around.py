@@ -297,3 +297,19 @@ def test_a_dropped_pools_memory_waits_for_a_side_stream(captured):
     assert not side.query()
     assert not set(held) & {t.data_ptr() for t in other}
     torch.cuda.synchronize()
+
+
+def test_a_refused_call_leaves_no_error_behind():
+    """What the library has reported is not found again by the next one who asks the runtime."""
+    import ctypes
+
+    from terraform_provider_iterative_amd import _build
+
+    runtime = ctypes.CDLL(_build.HIP_SO)
+    torch.cuda.synchronize()
+    assert runtime.hipGetLastError() == 0
+    lib = ops.hip()
+    with pytest.raises(ops.HipError, match="hipHostRegister"):  # of no memory
+        lib.check(lib.tpi_host_register(None, 0), "hipHostRegister")
+    assert runtime.hipGetLastError() == 0
+    assert torch.zeros(3, device="cuda").tolist() == [0.0] * 3
