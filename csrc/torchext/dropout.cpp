@@ -229,13 +229,17 @@ at::Tensor dropout_meta(TPI_DROPOUT_ARGS) { return empty_out(x, residual, dtype)
 
 // The operator as torch knows it: whatever a program does to its operators (tracing, wrapped
 // tensors, differentiation) finds it there.
-at::Tensor call(const at::Tensor& x, const std::optional<at::Tensor>& residual,
-                at::ScalarType dtype, const Mask& mask, const std::optional<at::Tensor>& used) {
+const auto& dropout_op() {
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("tpi::dropout", "")
                              .typed<at::Tensor(TPI_DROPOUT_ARGS)>();
-  return op.call(x, residual, dtype, mask.threshold, mask.scale, mask.seed, mask.number, mask.state,
-                 mask.first, mask.strides, used);
+  return op;
+}
+
+at::Tensor call(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                at::ScalarType dtype, const Mask& mask, const std::optional<at::Tensor>& used) {
+  return dropout_op().call(x, residual, dtype, mask.threshold, mask.scale, mask.seed, mask.number,
+                           mask.state, mask.first, mask.strides, used);
 }
 
 // A gradient has whatever layout the rest of the graph gave it.  One of more dimensions than a launch
@@ -286,9 +290,18 @@ at::Tensor tangent(const std::optional<at::Tensor>& t) {
 }
 
 at::Tensor dropout_autograd(TPI_DROPOUT_ARGS) {
-  const auto mask = c10::make_intrusive<Mask>(threshold, scale, seed, number, state, first, strides);
   const at::Tensor tx = tangent(x), tr = tangent(residual);
-  if ((tx.defined() || tr.defined()) && c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+  const bool forward =
+      (tx.defined() || tr.defined()) && c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  const bool backward =
+      at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad()));
+  if (!forward && !backward) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return dropout_op().call(x, residual, dtype, threshold, scale, seed, number, state, first, strides,
+                             used);
+  }
+  const auto mask = c10::make_intrusive<Mask>(threshold, scale, seed, number, state, first, strides);
+  if (forward) {
     // linear in both: the tangent is the operator, applied to x's, plus the residual's
     std::optional<at::Tensor> added, turned;
     if (residual) added = tr.defined() ? residual->_fw_primal(0) : *residual;
@@ -297,10 +310,7 @@ at::Tensor dropout_autograd(TPI_DROPOUT_ARGS) {
     return at::_make_dual(out, tx.defined() ? call(tx, turned, dtype, *mask, std::nullopt) : tr.clone(),
                           0);
   }
-  if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
-    return Dropout::apply(x, residual, dtype, mask, used);
-  const at::AutoDispatchBelowADInplaceOrView below;
-  return call(x, residual, dtype, *mask, used);
+  return Dropout::apply(x, residual, dtype, mask, used);
 }
 
 at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residual,
@@ -310,10 +320,9 @@ at::Tensor dropout(const at::Tensor& x, const std::optional<at::Tensor>& residua
   // views that are negated lazily (the imaginary part of a conjugate) are written out
   std::optional<at::Tensor> added;
   if (residual) added = residual->resolve_neg();
-  return call(x.resolve_neg(), added, added ? added->scalar_type() : x.scalar_type(),
-              Mask((int64_t)threshold, scale, (int64_t)seed, (int64_t)number, state, (int64_t)first,
-                   strides),
-              std::nullopt);
+  return dropout_op().call(x.resolve_neg(), added, added ? added->scalar_type() : x.scalar_type(),
+                           (int64_t)threshold, scale, (int64_t)seed, (int64_t)number, state,
+                           (int64_t)first, strides, std::nullopt);
 }
 
 TORCH_LIBRARY(tpi, m) {
