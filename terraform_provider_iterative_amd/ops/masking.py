@@ -53,8 +53,8 @@ class MaskStream:
     With ``device`` the seed and number are held there and read when a kernel runs, so that a
     captured graph draws new masks at every replay: call :meth:`advance` once per step, inside
     the capture, after the step's last draw.  A draw keeps its mask, also once the stream has
-    advanced (a block that the backward pass computes again).  Without it a capture is refused, because every
-    replay would repeat the captured masks; so are ``torch.jit.trace``, ``make_fx`` and
+    advanced (a block that the backward pass computes again).  Without it a capture is refused,
+    because every replay would repeat the captured masks; so are ``torch.jit.trace``, ``make_fx`` and
     ``torch.export`` (they record a draw that is given as numbers, ``torch.ops.tpi.dropout``).
     """
 

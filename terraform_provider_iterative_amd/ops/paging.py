@@ -49,8 +49,8 @@ def _pad4(words: int) -> int:
 
 
 def _has_memory(t: torch.Tensor) -> bool:
-    """Whether all elements lie in memory of the tensor's own: those of a wrapper (DTensor, fake, jagged)
-    or of a freed storage do not, and the kernels go by addresses."""
+    """Whether all elements lie in memory of the tensor's own: those of a wrapper (DTensor, fake,
+    jagged) or of a freed storage do not, and the kernels go by addresses."""
     if t.layout is not torch.strided or t.is_nested or torch._is_zerotensor(t):
         return False
     span = t.storage_offset() + 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
@@ -61,9 +61,9 @@ class PagePool:
     """The pages of ``tensors`` and the ``slots`` sequences that hold them.
 
     ``tensors``: one or more tensors of one device whose first dimension is the page, all with the
-    same number of pages and none sharing memory; a page's bytes are one contiguous run, or several with one stride
-    between them (``[heads, pages, ...]`` storage seen pages first).  ``page_tokens``: tokens
-    of a page.  ``width``: pages that one sequence can have (default: all).
+    same number of pages and none sharing memory; a page's bytes are one contiguous run, or
+    several with one stride between them (``[heads, pages, ...]`` storage seen pages first).
+    ``page_tokens``: tokens of a page.  ``width``: pages that one sequence can have (default: all).
 
     * :attr:`table` ``[slots, width]`` int32: pages of each slot's sequence, -1 behind its end
     * :attr:`lengths` ``[slots]`` int32: its tokens; 0: the slot is free
@@ -294,9 +294,9 @@ class PagePool:
 
     def copy(self, src: Numbers, dst: Numbers) -> None:
         """Page ``src[i]`` to page ``dst[i]`` in every tensor; sequences and counts stay as they are (of
-        a free page that is written, :meth:`compact` knows to clear it).  No page may be a destination twice, nor
-        destination and source: of such a call on device numbers, those destinations' content is
-        undefined.  A pair with a number out of range is left out."""
+        a free page that is written, :meth:`compact` knows to clear it).  No page may be a
+        destination twice, nor destination and source: of such a call on device numbers, those
+        destinations' content is undefined.  A pair with a number out of range is left out."""
         known = not self._on_device or not (isinstance(src, torch.Tensor) or
                                                   isinstance(dst, torch.Tensor))
         if known and set(map(int, src)) & set(map(int, dst)):
