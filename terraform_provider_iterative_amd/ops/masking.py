@@ -67,15 +67,22 @@ class MaskStream:
                                       device=device)
             self._ahead = 0
             self._copies: dict = {}
+            self._replayed = False  # a graph or a recorded program advances the state by itself
+
+    def _where(self) -> Tuple[int, int]:
+        """The stream that a kernel would go to, and the capture (0: none)."""
+        return torch_hip().stream_and_capture(self.state.device.index) if self.state.is_cuda else (0, 0)
 
     def _copy(self, recorded: int) -> torch.Tensor:
         """What this step's draws refer to: a copy of the state, which advancing does not change.  One
-        for each stream and each captured graph that draws, ordered before what it draws."""
-        where = torch_hip().stream_and_capture(self.state.device.index) if self.state.is_cuda else 0
-        copy = None if recorded else self._copies.get(where)
+        for each stream and each captured graph that draws, ordered before what it draws; where the
+        state may have moved between two draws, one for each."""
+        where = self._where()
+        keep = not recorded and (where[1] or not self._replayed)
+        copy = self._copies.get(where) if keep else None
         if copy is None:
             copy = self.state + 0  # a kernel
-            if type(copy) is torch.Tensor and not recorded:  # a fake one is not kept, either
+            if keep and type(copy) is torch.Tensor:  # not a fake one
                 self._copies[where] = copy
         return copy
 
@@ -124,6 +131,8 @@ class MaskStream:
         """End of a step (device streams): the next step's draws come after this one's."""
         if self.state is None:
             raise ValueError("advance() is for a MaskStream with a device")
+        if self._where()[1] or torch_ext().surroundings() & _RECORDED:
+            self._replayed = True
         self.state[1:].add_(self._ahead)
         self._ahead, self._copies = 0, {}
 

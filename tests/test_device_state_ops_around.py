@@ -313,3 +313,21 @@ def test_a_refused_call_leaves_no_error_behind():
         lib.check(lib.tpi_host_register(None, 0), "hipHostRegister")
     assert runtime.hipGetLastError() == 0
     assert torch.zeros(3, device="cuda").tolist() == [0.0] * 3
+
+
+def test_draws_between_replays_follow_the_state():
+    """A replay advances the state without the stream's knowing: an eager draw after it, also of a step
+    that has drawn before it, has the number that state_dict() names."""
+    masks, x = ops.MaskStream(5, device="cuda"), torch.ones(512, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = ops.dropout(x, 0.5, masks)
+        masks.advance()
+    for _ in range(3):
+        for _ in range(2):
+            number = masks.state_dict()["number"]
+            assert torch.equal(ops.dropout(x, 0.5, masks), ops.dropout(x, 0.5, (5, number)))
+            start = int(masks.state[1])
+            graph.replay()
+            assert torch.equal(a, ops.dropout(x, 0.5, (5, start)))
+        masks.advance()

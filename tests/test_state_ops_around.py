@@ -668,3 +668,31 @@ def test_two_threads_compute_one_block_again_at_once():
     for t in threads:
         t.join()
     assert got[0] == got[1] == drawn and masks.number == 4
+
+
+def test_draws_between_runs_of_a_recorded_step_follow_the_state():
+    """The recorded program advances the state without the stream's knowing."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    masks, x = ops.MaskStream(3, device="cpu"), torch.ones(300)
+
+    def step(v):
+        out = ops.dropout(v, 0.5, masks)
+        masks.advance()
+        return out
+
+    recorded = make_fx(step)(x)
+    for _ in range(3):
+        for _ in range(2):
+            number = masks.state_dict()["number"]
+            assert torch.equal(ops.dropout(x, 0.5, masks), ops.dropout(x, 0.5, (3, number)))
+        masks.advance()
+        number = masks.state_dict()["number"]
+        assert torch.equal(recorded(x), ops.dropout(x, 0.5, (3, number)))
+        assert masks.state_dict()["number"] == number + 1
+        number = masks.state_dict()["number"]
+        assert torch.equal(ops.dropout(x, 0.5, masks), ops.dropout(x, 0.5, (3, number)))
+        recorded(x)
+        number = masks.state_dict()["number"]
+        assert torch.equal(ops.dropout(x, 0.5, masks), ops.dropout(x, 0.5, (3, number)))
+        masks.advance()
